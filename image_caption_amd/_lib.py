@@ -85,6 +85,36 @@ class AttnBwdDesc(C.Structure):
     ]
 
 
+class AttnWindowDesc(C.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("o", c_void_p),
+        ("q_bs", c_long), ("q_hs", c_long), ("q_ss", c_long),
+        ("k_bs", c_long), ("k_hs", c_long), ("k_ss", c_long),
+        ("v_bs", c_long), ("v_hs", c_long), ("v_ss", c_long),
+        ("o_bs", c_long), ("o_hs", c_long), ("o_ss", c_long),
+        ("dtype", c_int),
+        ("B", c_int), ("H", c_int), ("Hkv", c_int), ("S", c_int), ("hd", c_int),
+        ("q_start", c_int), ("nq", c_int),
+        ("window", c_int), ("prefix_len", c_int), ("prefix_open", c_int),
+        ("lens", c_void_p),
+        ("drop", Dropout),
+        ("lse", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_long),
+    ]
+
+
+class AttnWindowBwdDesc(C.Structure):
+    _fields_ = [
+        ("fwd", AttnWindowDesc),
+        ("dout", c_void_p), ("do_bs", c_long), ("do_hs", c_long), ("do_ss", c_long),
+        ("dq", c_void_p), ("dq_bs", c_long), ("dq_hs", c_long), ("dq_ss", c_long),
+        ("dk", c_void_p), ("dk_bs", c_long), ("dk_hs", c_long), ("dk_ss", c_long),
+        ("dv", c_void_p), ("dv_bs", c_long), ("dv_hs", c_long), ("dv_ss", c_long),
+        ("dq_scale", c_float),
+        ("delta", c_void_p),
+    ]
+
+
 class BlockParams(C.Structure):
     _fields_ = [(n, c_void_p) for n in (
         "norm1_w", "norm1_b", "in_proj_w", "in_proj_b", "out_proj_w", "out_proj_b", "norm2_w", "norm2_b",
@@ -143,6 +173,12 @@ SIGNATURES = {
     "capdec_attn_bwd": (c_int, [C.POINTER(AttnBwdDesc), c_void_p]),
     "capdec_attn_bwd_colsum_rows": (None, [c_int, c_int, c_int, c_int, C.POINTER(c_long), C.POINTER(c_long)]),
     "capdec_attn_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "capdec_attn_window_fwd_workspace": (c_long, [c_int] * 8),
+    "capdec_attn_window_fwd": (c_int, [C.POINTER(AttnWindowDesc), c_void_p]),
+    "capdec_attn_window_bwd_workspace": (c_long, [c_int] * 8),
+    "capdec_attn_window_bwd": (c_int, [C.POINTER(AttnWindowBwdDesc), c_void_p]),
+    "capdec_attn_window_decode_workspace": (c_long, [c_int] * 7),
+    "capdec_attn_window_decode": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p, c_int, c_int, c_void_p, c_long, c_void_p]),
     "capdec_logits_ce_workspace": (c_long, [c_long, c_int]),
     "capdec_logits_ce_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_long, c_long,
                                      c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,

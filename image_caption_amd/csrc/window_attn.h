@@ -1,0 +1,239 @@
+// Attention under a sliding window with first keys that stay visible: what its forward (window_fwd.hip) and backward
+// (window_bwd.hip) share -- the visibility rule, the row packing and the two matrix-core forms everything is made of.
+//
+// Rows.  The G = H / Hkv query heads that share a K/V head are packed into one row axis: row r = i * G + g is query i of
+// head hkv * G + g.  A tile of 32 (or 4 x 32) consecutive rows then shares every K/V tile it reads, one token with G heads
+// is the same case as G tokens with one head, and the gradients of a shared head are summed where they are formed.
+//
+// Visibility.  Key j of a query at position i in a sequence of n rows: two intervals of j,
+//     j < a  or  lo <= j < hi,   hi = min(i + 1, n), lo = i - window + 1, a = min(prefix, open ? n : hi),
+// all empty when i >= n.  Only key tiles that meet one of them are visited, and only tiles that are not wholly inside one
+// of them for every row pay for element masks.
+//
+// Matrix-core forms (32x32 accumulators: lane l holds column l & 31, rows 8 (e >> 2) + 4 (l >> 5) + (e & 3), e = 0..15):
+//   mma_rows  acc[x][y] += sum_d  L[x][d] f[y][d]    L: 32 rows in LDS, f: one row per lane in registers
+//   mma_cols  acc[d][y] += sum_x  L[x][d] p[x][y]    p: an accumulator of the first kind, used as it lies: the reduction
+//             index of this product may run in any order as long as both operands agree, and the order in which a lane
+//             holds x is such an order -- the transposing LDS read (bf16) or a strided one (f32) follows it.
+// So scores, probabilities and their gradients never leave the registers.
+#pragma once
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+struct WinArgs {
+    const void* q; const void* k; const void* v; void* o;
+    long q_bs, q_hs, q_ss, k_bs, k_hs, k_ss, v_bs, v_hs, v_ss, o_bs, o_hs, o_ss;
+    int B, H, Hkv, G, S, nq, q_start, last;      // last: the one query of sequence b sits at its last position, lens[b] - 1
+    unsigned g_magic;                            // floor(2^32 / G) + 1
+    int rows;                                    // nq * G
+    int window, prefix, open;                    // window: 1 << 30 for "no limit"
+    const int32_t* lens;
+    uint32_t drop_thr, drop_k0, drop_k1; float drop_scale; int S4;
+    float* lse;                                  // [B][H][nq] or null
+    int tiles, nsplit; float* part_o; float* part_ml;
+    // backward
+    const void* dout; long do_bs, do_hs, do_ss;
+    void* dq; long dq_bs, dq_hs, dq_ss;
+    void* dk; long dk_bs, dk_hs, dk_ss;
+    void* dv; long dv_bs, dv_hs, dv_ss;
+    float dq_scale; float* delta;
+    int ktiles, kp, ncp, ncn; float* part;       // key tiles, those that meet the prefix, chunks of either kind, their partial sums
+};
+
+constexpr float WIN_LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ int win_len(const WinArgs& p, int b) { return p.lens ? min(max(p.lens[b], 0), p.S) : p.S; }
+__device__ __forceinline__ int win_row_query(const WinArgs& p, int r) { return p.G == 1 ? r : (int)__umulhi((unsigned)r, p.g_magic); }
+
+// the two intervals of visible keys of a query at position pos
+struct WinSpan { int a, lo, hi; };
+__device__ __forceinline__ WinSpan win_span(const WinArgs& p, int pos, int n) {
+    WinSpan s;
+    const bool live = pos < n;
+    s.hi = live ? min(pos + 1, n) : 0;
+    s.lo = max(0, pos - p.window + 1);
+    s.a = live ? min(p.prefix, p.open ? n : s.hi) : 0;
+    return s;
+}
+// (bitwise, and used in selects only: a branch per element costs more, and a conditional store into a vector's element has
+// come out of the compiler without the store)
+__device__ __forceinline__ bool win_sees(const WinSpan& s, int key) { return (key < s.a) | ((key >= s.lo) & (key < s.hi)); }
+
+// workgroups b, b + 8, ... share an XCD: each XCD takes a contiguous run of logical ids, so neighbours in the grid (tiles that
+// read the same keys) share an L2
+__device__ __forceinline__ int win_xcd_id(int w, int n) {
+    const int per = n >> 3, rem = n & 7, xcd = w & 7;
+    return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (w >> 3);
+}
+
+template <typename T, int HD> struct WinGeo {
+    static constexpr int PB = HD * (int)sizeof(T) + 16;          // LDS bytes per row: an odd number of 16-byte units
+    static constexpr int CPR = HD * (int)sizeof(T) / 16;         // 16-byte chunks per row
+    static constexpr int DT = HD / 32;
+};
+
+// one row per lane (row = lane & 31; the two halves of the wave hold alternate pieces of it), as mma_rows wants it
+template <typename T, int HD> struct RowFrag;
+template <int HD> struct RowFrag<bf16_t, HD> {
+    bf16x8 f[HD / 16];
+    __device__ __forceinline__ void load(const bf16_t* row, int lane) {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) f[s] = *reinterpret_cast<const bf16x8*>(row + 16 * s + 8 * (lane >> 5));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) f[s] = __builtin_bit_cast(bf16x8, (u32x4{0, 0, 0, 0}));
+    }
+    // sum over this lane's half of the row
+    __device__ __forceinline__ float dot(const RowFrag& o) const {
+        float a = 0.f;
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a = fmaf((float)f[s][e], (float)o.f[s][e], a);
+        return a;
+    }
+};
+template <int HD> struct RowFrag<float, HD> {
+    f32x4 f[HD / 8];
+    __device__ __forceinline__ void load(const float* row, int lane) {
+#pragma unroll
+        for (int s = 0; s < HD / 8; ++s) f[s] = *reinterpret_cast<const f32x4*>(row + 8 * s + 4 * (lane >> 5));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int s = 0; s < HD / 8; ++s) f[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ float dot(const RowFrag& o) const {
+        float a = 0.f;
+#pragma unroll
+        for (int s = 0; s < HD / 8; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a = fmaf(f[s][e], o.f[s][e], a);
+        return a;
+    }
+};
+
+template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<bf16_t, HD>& b, int lane) {
+    const char* at = lds + (lane & 31) * WinGeo<bf16_t, HD>::PB + (lane >> 5) * 16;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(at + 32 * s), b.f[s], acc, 0, 0, 0);
+}
+template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<float, HD>& b, int lane) {
+    const char* at = lds + (lane & 31) * WinGeo<float, HD>::PB + (lane >> 5) * 16;
+#pragma unroll
+    for (int s = 0; s < HD / 8; ++s) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(at + 32 * s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b.f[s][e], acc, 0, 0, 0);
+    }
+}
+
+// p is rounded to bf16 (half a step, 2^-9 of each term) to be an operand: the products' own inputs have no more bits
+template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, bf16_t, int lane) {
+    constexpr int PB = WinGeo<bf16_t, HD>::PB;
+    const int g = lane >> 4, i = lane & 15;
+    const char* at = lds + (4 * (g >> 1) + (i >> 2)) * PB + (16 * (g & 1) + 4 * (i & 3)) * 2;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        bf16x8 pb;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pb[e] = (bf16_t)p[8 * c + e];
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) {
+            const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at + (16 * c) * PB + 64 * dt));
+            const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at + (16 * c + 8) * PB + 64 * dt));
+            const bf16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb, acc[dt], 0, 0, 0);
+        }
+    }
+}
+template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, float, int lane) {
+    constexpr int PB = WinGeo<float, HD>::PB;
+    const char* at = lds + 4 * (lane >> 5) * PB + (lane & 31) * 4;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(at + (8 * (e >> 2) + (e & 3)) * PB + 128 * dt), p[e], acc[dt], 0, 0, 0);
+}
+
+// NROWS rows of two strided matrices on their way to LDS; rows past the end arrive as zeros and are not read
+template <typename T, int HD, int NROWS, int NT> struct TilePair {
+    static constexpr int CPR = WinGeo<T, HD>::CPR, U = NROWS * CPR / NT;
+    static_assert(NROWS * CPR % NT == 0, "a tile is whole rounds of 16-byte loads");
+    u32x4 a[U], b[U];
+    __device__ __forceinline__ void fetch(const char* base0, unsigned ss0, const char* base1, unsigned ss1, int nvalid, int tid) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
+            a[j] = b[j] = u32x4{0, 0, 0, 0};
+            if (row < nvalid) {
+                a[j] = *reinterpret_cast<const u32x4*>(base0 + (unsigned)row * ss0 + ch * 16);
+                b[j] = *reinterpret_cast<const u32x4*>(base1 + (unsigned)row * ss1 + ch * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void commit(char* lds0, char* lds1, int tid) const {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
+            *reinterpret_cast<u32x4*>(lds0 + row * WinGeo<T, HD>::PB + ch * 16) = a[j];
+            *reinterpret_cast<u32x4*>(lds1 + row * WinGeo<T, HD>::PB + ch * 16) = b[j];
+        }
+    }
+};
+
+// the key tiles (BK keys each) that rows at positions p0..p1 can see: tiles 0..ns-1, then ws.., nt in all
+struct WinTiles {
+    int ns, ws, nt;
+    __device__ __forceinline__ int at(int idx) const { return idx < ns ? idx : ws + idx - ns; }
+};
+template <int BK> __device__ __forceinline__ WinTiles win_tiles(const WinArgs& p, int p0, int p1, int n) {
+    WinTiles t{0, 0, 0};
+    if (p0 >= n) return t;
+    const int hi = min(p1 + 1, n), lo = max(0, p0 - p.window + 1), a = min(p.prefix, p.open ? n : hi);
+    t.ns = (a + BK - 1) / BK;
+    t.ws = max(t.ns, lo / BK);
+    t.nt = t.ns + max(0, (hi + BK - 1) / BK - t.ws);
+    return t;
+}
+
+// four consecutive values d0 + 8 jj + 4 h .. of this lane's row from accumulator e = 4 jj .. 4 jj + 3; in bf16 the two halves
+// of the wave swap pieces so that a lane stores 16 bytes
+template <int HD> __device__ __forceinline__ void store_rows(const f32x16 (&acc)[HD / 32], float scale, float* row, bool ok, int lane) {
+    if (!ok) return;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+            *reinterpret_cast<f32x4*>(row + 32 * dt + 8 * jj + 4 * (lane >> 5)) =
+                f32x4{acc[dt][4 * jj] * scale, acc[dt][4 * jj + 1] * scale, acc[dt][4 * jj + 2] * scale, acc[dt][4 * jj + 3] * scale};
+}
+__device__ __forceinline__ unsigned win_pack(float a, float b) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    bf16x2 t;
+    t[0] = (bf16_t)a; t[1] = (bf16_t)b;
+    return __builtin_bit_cast(unsigned, t);
+}
+template <int HD> __device__ __forceinline__ void store_rows(const f32x16 (&acc)[HD / 32], float scale, bf16_t* row, bool ok, int lane) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+            const unsigned x0 = win_pack(acc[dt][8 * jp] * scale, acc[dt][8 * jp + 1] * scale), x1 = win_pack(acc[dt][8 * jp + 2] * scale, acc[dt][8 * jp + 3] * scale);
+            const unsigned y0 = win_pack(acc[dt][8 * jp + 4] * scale, acc[dt][8 * jp + 5] * scale), y1 = win_pack(acc[dt][8 * jp + 6] * scale, acc[dt][8 * jp + 7] * scale);
+            const u32x2 s0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false);
+            const u32x2 s1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+            // lower half: columns 16 jp .. + 7 (its own four and the upper half's four), upper half: 16 jp + 8 ..
+            if (ok) *reinterpret_cast<u32x4*>(row + 32 * dt + 16 * jp + 8 * (lane >> 5)) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+        }
+}
+
+// ------------------------------------------------------------------ host side
+int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what);
+struct WinFwdPlan { int kw; int tiles; int nsplit; long part_floats; };   // kw: four waves share the keys of 32 rows (else 4 x 32 rows)
+WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix);
+int win_fwd_launch(WinArgs& a, int dtype, int hd, void* workspace, long workspace_bytes, hipStream_t st);

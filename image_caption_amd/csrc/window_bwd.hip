@@ -1,0 +1,475 @@
+// Backward of attention under a sliding window with first keys that stay visible (rule and shared pieces: window_attn.h).
+//
+//     P = exp(S - lse),  delta = sum_d dO O,  dP = dO V^T,  dS = P (dP - delta),
+//     dQ = dS K,   dK = dS^T Q,   dV = P^T dO            (q carries its scale; dq is multiplied by dq_scale)
+//
+// Two kernels, each recomputing P from the saved log-sum-exp: one owns query rows and walks the key tiles they see (dQ, and
+// delta on its way), one owns 128 keys and walks the rows that see them (dK, dV; the heads that share a K/V head are
+// neighbouring rows, so their sum needs nothing more).  Seven products where five would do, but no atomics: every sum is
+// formed in a fixed order.
+//
+// Keys of the prefix are seen by every row, the others by window + 128 positions: a prefix tile's rows are cut into chunks
+// that leave f32 partial sums in the workspace, added in order by a third kernel.
+#include "window_attn.h"
+
+namespace {
+
+constexpr int KT = 128;              // keys of a dK / dV workgroup: four waves of 32
+constexpr int RB = 32;               // rows per step
+
+// ------------------------------------------------------------------ dQ (and delta)
+template <typename T, int HD, int QW, int KW, bool DROP>
+__global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_kernel(WinArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using G = WinGeo<T, HD>;
+    constexpr int NSUB = KW == 1 && sizeof(T) == 2 ? 2 : 1;
+    constexpr int NT = 64 * QW * KW, BK = 32 * KW * NSUB, NBUF = KW == 1 ? 2 : 1;
+    constexpr int MAT = BK * G::PB;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
+    const int id = win_xcd_id(blockIdx.x, gridDim.x);
+    const int tile = id % p.tiles, bh = id / p.tiles;
+    const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
+    const int n = win_len(p, b), q0 = p.q_start;
+    const int r_first = tile * 32 * QW, r_end = min(p.rows, r_first + 32 * QW);
+    const WinTiles tl = win_tiles<BK>(p, q0 + win_row_query(p, r_first), q0 + win_row_query(p, r_end - 1), n);
+
+    const int w_first = r_first + 32 * qw;
+    const int r = w_first + (lane & 31), rc = min(r, p.rows - 1);
+    const int irel = win_row_query(p, rc), head = hkv * p.G + rc - irel * p.G, pos = q0 + irel;
+    const WinSpan sp = win_span(p, pos, n);
+    const int wp0 = q0 + win_row_query(p, min(w_first, p.rows - 1)), wp1 = q0 + win_row_query(p, min(w_first + 31, p.rows - 1));
+    const WinSpan s0 = win_span(p, wp0, n), s1 = win_span(p, wp1, n);
+    const bool all_live = wp1 < n;
+    const int any_hi = all_live ? s1.hi : (wp0 < n ? n : 0);
+    const int any_a = p.open ? max(s0.a, s1.a) : min(p.prefix, any_hi);
+    const int any_end = w_first < p.rows ? max(any_a, any_hi) : 0;
+
+    RowFrag<T, HD> qf, df;
+    const long stat = ((long)b * p.H + head) * p.nq + irel;
+    float lse = INFINITY, delta = 0.f;
+    qf.zero();
+    df.zero();
+    if (pos < n) {                     // (a row past its sequence's end holds nothing that may be read into a sum)
+        RowFrag<T, HD> of;
+        qf.load(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)head * p.q_hs + (long)irel * p.q_ss, lane);
+        df.load(reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)head * p.do_hs + (long)irel * p.do_ss, lane);
+        of.load(reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)head * p.o_hs + (long)irel * p.o_ss, lane);
+        delta = df.dot(of);
+        lse = p.lse[stat];
+        if (lse == -INFINITY) lse = INFINITY;          // a row that sees nothing: every probability is 0
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (kw == 0 && r < p.rows && lane < 32) p.delta[stat] = delta;
+
+    f32x16 acc[G::DT];
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+
+    const char* kbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs);
+    const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
+    const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
+    const float lsel = lse * WIN_LOG2E;
+    TilePair<T, HD, BK, NT> tp;
+    auto fetch = [&](int idx) {
+        const int key0 = tl.at(idx) * BK;
+        tp.fetch(kbase + key0 * kss, (unsigned)kss, vbase + key0 * vss, (unsigned)vss, n - key0, tid);
+    };
+    auto compute = [&](int idx, const char* lk0, const char* lv0) {
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+            const int at = kw * 32 * NSUB + 32 * u, key0 = tl.at(idx) * BK + at;
+            if (key0 >= any_end || (key0 >= any_a && key0 + 32 <= s0.lo)) continue;
+            const char* lk = lk0 + at * G::PB;
+            const char* lv = lv0 + at * G::PB;
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+            mma_rows<HD>(s, lk, qf, lane);
+            mma_rows<HD>(dp, lv, df, lane);
+            const bool whole = all_live && (key0 + 32 <= s0.a || (key0 >= s1.lo && key0 + 32 <= s0.hi));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = sizeof(T) == 2 ? fmaf(s[e], WIN_LOG2E, -lsel) : (s[e] - lse) * WIN_LOG2E;
+                s[e] = __builtin_amdgcn_exp2f(x);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = win_sees(sp, key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) ? s[e] : 0.f;
+            }
+            if constexpr (DROP) {
+                const uint32_t row = (uint32_t)((((long)b * p.H + head) * p.S + pos) * p.S4) + (uint32_t)(key0 + 4 * (lane >> 5));
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    bool keep[4];
+                    dropout_keep4(p.drop_k0, p.drop_k1, row + 8 * jj, p.drop_thr, keep);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * jj + e] = keep[e] ? dp[4 * jj + e] * p.drop_scale : 0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
+            mma_cols<HD>(acc, lk, s, T{}, lane);
+        }
+    };
+    if (tl.nt > 0) {
+        fetch(0);
+        if constexpr (NBUF == 2) {
+            tp.commit(smem, smem + MAT, tid);
+            __syncthreads();
+            for (int idx = 0; idx < tl.nt; ++idx) {
+                const int cur = idx & 1;
+                const bool more = idx + 1 < tl.nt;
+                if (more) fetch(idx + 1);
+                compute(idx, smem + 2 * cur * MAT, smem + (2 * cur + 1) * MAT);
+                if (more) tp.commit(smem + 2 * (cur ^ 1) * MAT, smem + (2 * (cur ^ 1) + 1) * MAT, tid);
+                __syncthreads();
+            }
+        } else {
+            for (int idx = 0; idx < tl.nt; ++idx) {
+                tp.commit(smem, smem + MAT, tid);
+                __syncthreads();
+                if (idx + 1 < tl.nt) fetch(idx + 1);
+                compute(idx, smem, smem + MAT);
+                __syncthreads();
+            }
+        }
+    }
+    if constexpr (KW == 1) {
+        T* out = reinterpret_cast<T*>(p.dq) + (long)b * p.dq_bs + (long)head * p.dq_hs + (long)irel * p.dq_ss;
+        store_rows<HD>(acc, p.dq_scale, out, r < p.rows, lane);
+    } else {
+        constexpr int PJ = HD + 4;
+        float* jo = reinterpret_cast<float*>(smem);
+        store_rows<HD>(acc, p.dq_scale, jo + (kw * 32 + (lane & 31)) * PJ, true, lane);
+        __syncthreads();
+        for (int u = tid; u < 32 * HD / 4; u += NT) {
+            const int row = u / (HD / 4), c = (u - row * (HD / 4)) * 4, rr = r_first + row;
+            if (rr >= p.rows) break;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < KW; ++w) v += *reinterpret_cast<const f32x4*>(jo + (w * 32 + row) * PJ + c);
+            const int i = win_row_query(p, rr), h = hkv * p.G + rr - i * p.G;
+            T* at = reinterpret_cast<T*>(p.dq) + (long)b * p.dq_bs + (long)h * p.dq_hs + (long)i * p.dq_ss + c;
+            if constexpr (sizeof(T) == 2) {
+                bf16x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (bf16_t)v[e];
+                *reinterpret_cast<bf16x4*>(at) = w;
+            } else {
+                *reinterpret_cast<f32x4*>(at) = v;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ dK, dV
+// rows (relative to the packed axis) that see a key of tile k0..k0+KT-1: blocks of RB rows [first, first + count)
+struct RowBlocks { int first, count; };
+__device__ __forceinline__ RowBlocks win_row_blocks(const WinArgs& p, int k0, int n) {
+    if (k0 >= n) return {0, 0};
+    const bool pre = k0 < p.prefix;
+    const int lo = pre && p.open ? 0 : k0;
+    const long far = (long)k0 + KT - 1 + p.window;                                  // first position past the window of the tile's last key
+    const int hi = pre ? n : (int)min((long)n, far);
+    const int i0 = max(0, lo - p.q_start), i1 = min(p.nq, hi - p.q_start);
+    if (i1 <= i0) return {0, 0};
+    const int first = i0 * p.G / RB;
+    return {first, (i1 * p.G + RB - 1) / RB - first};
+}
+
+template <typename T, int HD, bool DROP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(WinArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using G = WinGeo<T, HD>;
+    constexpr int CPR = G::CPR, U = (RB * CPR + 255) / 256;
+    constexpr int MAT = RB * G::PB;
+    // [2 buffers] { Q, dO, 32 lse, 32 delta, 32 positions }
+    constexpr int BUF = 2 * MAT + 3 * RB * 4;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int per_bh = p.kp * p.ncp + (p.ktiles - p.kp) * p.ncn;
+    const int id = win_xcd_id(blockIdx.x, gridDim.x);
+    const int bh = id / per_bh, in = id - bh * per_bh;
+    int tile, chunk, nc, slot;
+    if (in < p.kp * p.ncp) { tile = in / p.ncp; chunk = in - tile * p.ncp; nc = p.ncp; slot = in; }
+    else {
+        const int x = in - p.kp * p.ncp;
+        tile = p.kp + x / p.ncn; chunk = x % p.ncn; nc = p.ncn;
+        slot = (p.ncp > 1 ? p.kp * p.ncp : 0) + x;
+    }
+    const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
+    const int n = win_len(p, b);
+    const int k0 = tile * KT, kw0 = k0 + 32 * wave, key = kw0 + (lane & 31);
+    const RowBlocks rb = win_row_blocks(p, k0, n);
+    const int b_begin = rb.first + (int)((long)rb.count * chunk / nc), b_end = rb.first + (int)((long)rb.count * (chunk + 1) / nc);
+
+    RowFrag<T, HD> kf, vf;
+    kf.zero();
+    vf.zero();
+    if (key < n) {
+        kf.load(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)key * p.k_ss, lane);
+        vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+    }
+    f32x16 dk[G::DT], dv[G::DT];
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+
+    u32x4 fq[U], fd[U];
+    float f_lse = INFINITY, f_delta = 0.f;
+    int f_pos = 0;
+    auto fetch = [&](int blk) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR, r = blk * RB + row;
+            fq[j] = fd[j] = u32x4{0, 0, 0, 0};
+            if (row < RB && r < p.rows) {
+                const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
+                if (p.q_start + i < n) {
+                    fq[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i * p.q_ss + ch * (16 / (int)sizeof(T)));
+                    fd[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)h * p.do_hs + (long)i * p.do_ss + ch * (16 / (int)sizeof(T)));
+                }
+            }
+        }
+        if (tid < RB) {
+            const int r = blk * RB + tid, rc = min(r, p.rows - 1), i = win_row_query(p, rc), h = hkv * p.G + rc - i * p.G;
+            f_pos = p.q_start + i;
+            f_lse = INFINITY;                         // rows that are not there, and rows that see nothing: probability 0
+            f_delta = 0.f;
+            if (r < p.rows && f_pos < n) {
+                const long stat = ((long)b * p.H + h) * p.nq + i;
+                const float v = p.lse[stat];
+                f_lse = v == -INFINITY ? INFINITY : v;
+                f_delta = p.delta[stat];
+            }
+        }
+    };
+    auto commit = [&](char* buf) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            if (row < RB) {
+                *reinterpret_cast<u32x4*>(buf + row * G::PB + ch * 16) = fq[j];
+                *reinterpret_cast<u32x4*>(buf + MAT + row * G::PB + ch * 16) = fd[j];
+            }
+        }
+        if (tid < RB) {
+            float* st = reinterpret_cast<float*>(buf + 2 * MAT);
+            st[tid] = f_lse;
+            st[RB + tid] = f_delta;
+            reinterpret_cast<int*>(st)[2 * RB + tid] = f_pos;
+        }
+    };
+    auto compute = [&](int blk, const char* buf) {
+        const int ra = blk * RB, rz = min(p.rows, ra + RB) - 1;
+        const int pf = p.q_start + win_row_query(p, ra), pl = p.q_start + win_row_query(p, rz);
+        const bool pre = kw0 < p.prefix;
+        const bool band = pl >= kw0 && pf - p.window < kw0 + 31;
+        if (kw0 >= n || !(band || (pre && (p.open || pl >= kw0)))) return;
+        f32x16 s, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+        mma_rows<HD>(s, buf, kf, lane);
+        mma_rows<HD>(dp, buf + MAT, vf, lane);
+        const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
+        const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * jj);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = sizeof(T) == 2 ? fmaf(s[4 * jj + e], WIN_LOG2E, -lse[e] * WIN_LOG2E) : (s[4 * jj + e] - lse[e]) * WIN_LOG2E;
+                s[4 * jj + e] = __builtin_amdgcn_exp2f(x);
+            }
+        }
+        if (!whole) {
+            const int* ps0 = reinterpret_cast<const int*>(st) + 2 * RB;
+            // key <= pos and pos < far, or (a key of the prefix) pos >= near: two intervals of positions per lane
+            const int far = key < n ? key + p.window : 0;                                  // (window <= 2^30, key < 2^28)
+            const int near = key < min(p.prefix, n) ? (p.open ? 0 : key) : 0x7FFFFFFF;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int pos = ps0[8 * jj + e];
+                    s[4 * jj + e] = ((pos >= near) | ((pos >= key) & (pos < far))) ? s[4 * jj + e] : 0.f;
+                }
+        }
+        f32x16 pd = s;                                // what multiplies dO: the probabilities after dropout
+        if constexpr (DROP) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = min(ra + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), p.rows - 1);
+                const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
+                const uint32_t at = (uint32_t)((((long)b * p.H + h) * p.S + p.q_start + i) * p.S4) + (uint32_t)key;
+                const float f = dropout_keep(p.drop_k0, p.drop_k1, at, p.drop_thr) ? p.drop_scale : 0.f;
+                pd[e] *= f;
+                dp[e] *= f;
+            }
+        }
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(st + RB + 8 * jj);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * jj + e] *= dp[4 * jj + e] - delta[e];
+        }
+        mma_cols<HD>(dv, buf + MAT, pd, T{}, lane);
+        mma_cols<HD>(dk, buf, s, T{}, lane);
+    };
+    if (b_begin < b_end) {
+        fetch(b_begin);
+        commit(smem);
+        __syncthreads();
+        for (int blk = b_begin; blk < b_end; ++blk) {
+            const int cur = (blk - b_begin) & 1;
+            const bool more = blk + 1 < b_end;
+            if (more) fetch(blk + 1);
+            compute(blk, smem + cur * BUF);
+            if (more) commit(smem + (cur ^ 1) * BUF);
+            __syncthreads();
+        }
+    }
+    if (nc == 1) {
+        const bool ok = key < p.S;
+        store_rows<HD>(dk, 1.f, reinterpret_cast<T*>(p.dk) + (long)b * p.dk_bs + (long)hkv * p.dk_hs + (long)min(key, p.S - 1) * p.dk_ss, ok, lane);
+        store_rows<HD>(dv, 1.f, reinterpret_cast<T*>(p.dv) + (long)b * p.dv_bs + (long)hkv * p.dv_hs + (long)min(key, p.S - 1) * p.dv_ss, ok, lane);
+    } else {
+        const long slots = (p.ncp > 1 ? p.kp * p.ncp : 0) + (p.ncn > 1 ? (p.ktiles - p.kp) * p.ncn : 0);
+        float* at = p.part + ((bh * slots + slot) * 2L * KT + 32 * wave + (lane & 31)) * HD;
+        store_rows<HD>(dk, 1.f, at, true, lane);
+        store_rows<HD>(dv, 1.f, at + (long)KT * HD, true, lane);
+    }
+}
+
+// dK and dV of the tiles that were cut into chunks: the partial sums in chunk order.  Grid: (column pieces of a tile, cut tiles, B * Hkv)
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
+    const int x = blockIdx.y, bh = blockIdx.z;
+    const int np = p.ncp > 1 ? p.kp : 0;
+    const int tile = x < np ? x : p.kp + (x - np), nc = x < np ? p.ncp : p.ncn;
+    const long slots = (p.ncp > 1 ? p.kp * p.ncp : 0) + (p.ncn > 1 ? (p.ktiles - p.kp) * p.ncn : 0);
+    const long slot0 = x < np ? (long)x * p.ncp : (long)np * p.ncp + (long)(x - np) * p.ncn;
+    const int u = blockIdx.x * 256 + threadIdx.x;                         // four columns of dK (first half) or dV
+    const int which = u / (KT * HD / 4), c4 = u - which * (KT * HD / 4);
+    const int row = c4 / (HD / 4), c = (c4 - row * (HD / 4)) * 4, key = tile * KT + row;
+    if (which > 1 || key >= p.S) return;
+    const float* at = p.part + ((bh * slots + slot0) * 2 + which) * (long)KT * HD + (long)row * HD + c;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < nc; ++s) v += *reinterpret_cast<const f32x4*>(at + (long)s * 2 * KT * HD);
+    const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
+    T* out = which == 0 ? reinterpret_cast<T*>(p.dk) + (long)b * p.dk_bs + (long)hkv * p.dk_hs + (long)key * p.dk_ss + c
+                        : reinterpret_cast<T*>(p.dv) + (long)b * p.dv_bs + (long)hkv * p.dv_hs + (long)key * p.dv_ss + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(v[e]);
+}
+
+// ------------------------------------------------------------------ launch
+struct BwdPlan { int ktiles, kp, ncp, ncn; long part_floats; };
+BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix) {
+    BwdPlan pl;
+    const int G = H / Hkv;
+    const long bh = (long)B * Hkv, rows = (long)nq * G;
+    pl.ktiles = (S + KT - 1) / KT;
+    const int pre = prefix < S ? prefix : S;
+    const long w = window == 0 || window > S ? S : window;
+    pl.kp = (pre + KT - 1) / KT;
+    const long all = (rows + RB - 1) / RB;                                 // row blocks a prefix tile sees
+    long band = ((w + KT) * G + RB - 1) / RB;                              // and another one
+    if (band > all) band = all;
+    // enough workgroups for two per CU, none with fewer than 16 steps for it
+    auto chunks = [](long wgs, long steps) {
+        long c = wgs > 0 ? (512 + wgs - 1) / wgs : 1;
+        if (c > steps / 16) c = steps / 16;
+        return (int)(c < 1 ? 1 : c);
+    };
+    pl.ncn = chunks(bh * pl.ktiles, band);
+    pl.ncp = pl.kp ? chunks(bh * pl.kp, all) : 1;
+    if (pl.ncp < pl.ncn) pl.ncp = pl.ncn;
+    const long slots = (pl.ncp > 1 ? (long)pl.kp * pl.ncp : 0) + (pl.ncn > 1 ? (long)(pl.ktiles - pl.kp) * pl.ncn : 0);
+    pl.part_floats = bh * slots * 2 * KT * hd;
+    return pl;
+}
+
+template <typename T, int HD, bool DROP>
+int bwd_go(WinArgs& a, hipStream_t st) {
+    using G = WinGeo<T, HD>;
+    const long bh = (long)a.B * a.Hkv;
+    {   // dQ: four waves on the keys of 32 rows when there are few rows
+        const bool kw = a.rows <= 64;
+        constexpr int NS = sizeof(T) == 2 ? 2 : 1;
+        a.tiles = (a.rows + (kw ? 31 : 127)) / (kw ? 32 : 128);
+        CAPDEC_CHECK(bh * a.tiles < (1L << 31), "attn_window_bwd: grid too large");
+        auto go = [&](auto kfn, int lds) {
+            if (lds > 64 * 1024) ensure_dynamic_lds((const void*)kfn, lds);
+            hipLaunchKernelGGL(kfn, dim3((unsigned)(bh * a.tiles)), dim3(256), lds, st, a);
+        };
+        constexpr int lds_q = 4 * 32 * NS * G::PB, lds_t = 2 * 128 * G::PB, lds_j = 4 * 32 * (HD + 4) * 4;
+        if (kw) go(win_dq_kernel<T, HD, 1, 4, DROP>, lds_t > lds_j ? lds_t : lds_j);
+        else go(win_dq_kernel<T, HD, 4, 1, DROP>, lds_q);
+        CAPDEC_LAUNCH_CHECK();
+    }
+    const long grid = bh * ((long)a.kp * a.ncp + (long)(a.ktiles - a.kp) * a.ncn);
+    CAPDEC_CHECK(grid < (1L << 31), "attn_window_bwd: grid too large");
+    auto kfn = win_dkv_kernel<T, HD, DROP>;
+    constexpr int lds = 2 * (2 * RB * G::PB + 3 * RB * 4);
+    if (lds > 64 * 1024) ensure_dynamic_lds((const void*)kfn, lds);
+    hipLaunchKernelGGL(kfn, dim3((unsigned)grid), dim3(256), lds, st, a);
+    CAPDEC_LAUNCH_CHECK();
+    const int cut = (a.ncp > 1 ? a.kp : 0) + (a.ncn > 1 ? a.ktiles - a.kp : 0);
+    if (cut > 0) {
+        hipLaunchKernelGGL((win_dkv_join_kernel<T, HD>), dim3((2 * KT * HD / 4 + 255) / 256, cut, (unsigned)bh), dim3(256), 0, st, a);
+        CAPDEC_LAUNCH_CHECK();
+    }
+    return CAPDEC_OK;
+}
+template <typename T, int HD> int bwd_hd(WinArgs& a, hipStream_t st) {
+    return a.drop_thr ? bwd_go<T, HD, true>(a, st) : bwd_go<T, HD, false>(a, st);
+}
+template <typename T> int bwd_type(WinArgs& a, int hd, hipStream_t st) {
+    switch (hd) {
+        case 32: return bwd_hd<T, 32>(a, st);
+        case 64: return bwd_hd<T, 64>(a, st);
+        case 96: return bwd_hd<T, 96>(a, st);
+        default: return bwd_hd<T, 128>(a, st);
+    }
+}
+
+}  // namespace
+
+extern "C" long capdec_attn_window_bwd_workspace(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix_len) {
+    if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || S <= 0 || nq <= 0 || hd <= 0 || window < 0 || prefix_len < 0) return 0;
+    return bwd_plan(B, H, Hkv, S, nq, hd, window, prefix_len).part_floats * 4;
+}
+
+extern "C" int capdec_attn_window_bwd(const capdec_attn_window_bwd_desc* d, void* stream) {
+    CAPDEC_CHECK(d != nullptr, "attn_window_bwd: null descriptor");
+    WinArgs a;
+    const int rc = win_fill(&d->fwd, a, "attn_window_bwd");
+    if (rc != CAPDEC_OK) return rc;
+    CAPDEC_CHECK(d->dout && d->dq && d->dk && d->dv && d->delta && a.lse, "attn_window_bwd: null pointer");
+    CAPDEC_CHECK(aligned16(d->dout) && aligned16(d->dq) && aligned16(d->dk) && aligned16(d->dv), "attn_window_bwd: operands must be 16-byte aligned");
+    const int per16 = d->fwd.dtype == CAPDEC_BF16 ? 8 : 4;
+    const long strides[] = {d->do_bs, d->do_hs, d->do_ss, d->dq_bs, d->dq_hs, d->dq_ss, d->dk_bs, d->dk_hs, d->dk_ss, d->dv_bs, d->dv_hs, d->dv_ss};
+    for (long s : strides) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "attn_window_bwd: stride %ld (must be a non-negative multiple of %d elements)", s, per16);
+    const BwdPlan pl = bwd_plan(a.B, a.H, a.Hkv, a.S, a.nq, d->fwd.hd, d->fwd.window, a.prefix);
+    CAPDEC_CHECK((long)a.B * a.Hkv < 65536 || pl.part_floats == 0, "attn_window_bwd: B * Hkv %ld", (long)a.B * a.Hkv);
+    if (pl.part_floats > 0) {
+        if (!d->fwd.workspace || d->fwd.workspace_bytes < pl.part_floats * 4) {
+            capdec_set_error("attn_window_bwd: workspace %ld bytes < %ld", d->fwd.workspace ? d->fwd.workspace_bytes : 0L, pl.part_floats * 4);
+            return CAPDEC_ERR_WORKSPACE;
+        }
+        CAPDEC_CHECK(aligned16(d->fwd.workspace), "attn_window_bwd: workspace must be 16-byte aligned");
+    }
+    a.dout = d->dout; a.do_bs = d->do_bs; a.do_hs = d->do_hs; a.do_ss = d->do_ss;
+    a.dq = d->dq; a.dq_bs = d->dq_bs; a.dq_hs = d->dq_hs; a.dq_ss = d->dq_ss;
+    a.dk = d->dk; a.dk_bs = d->dk_bs; a.dk_hs = d->dk_hs; a.dk_ss = d->dk_ss;
+    a.dv = d->dv; a.dv_bs = d->dv_bs; a.dv_hs = d->dv_hs; a.dv_ss = d->dv_ss;
+    a.dq_scale = d->dq_scale; a.delta = d->delta;
+    a.ktiles = pl.ktiles; a.kp = pl.kp; a.ncp = pl.ncp; a.ncn = pl.ncn; a.part = (float*)d->fwd.workspace;
+    return d->fwd.dtype == CAPDEC_BF16 ? bwd_type<bf16_t>(a, d->fwd.hd, (hipStream_t)stream) : bwd_type<float>(a, d->fwd.hd, (hipStream_t)stream);
+}

@@ -11,8 +11,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import (ACT_NONE, BF16, F32, GATE_NONE, MASK_NONE, NO_DROPOUT, AttnBwdDesc, AttnDesc, Dropout, GemmDesc,
-                   check, dtype_code, ptr, require_cuda, stream_ptr)
+from ._lib import (ACT_NONE, BF16, F32, GATE_NONE, MASK_NONE, NO_DROPOUT, AttnBwdDesc, AttnDesc, AttnWindowBwdDesc,
+                   AttnWindowDesc, Dropout, GemmDesc, check, dtype_code, ptr, require_cuda, stream_ptr)
 
 
 def _st():
@@ -285,6 +285,141 @@ def attn_decode(q, kv_cache, o, B, H, hd, smax, length):
     require_cuda(q, kv_cache, o)
     check(_lib.load().capdec_attn_decode(ptr(q), ptr(kv_cache), ptr(o), dtype_code(q), B, H, hd, smax, length, _st()),
           "capdec_attn_decode")
+
+
+def _need(cond: bool, what: str):
+    if not cond:
+        raise ValueError(what)
+
+
+def _on_current_device(*tensors):
+    """The launch goes to the current device's current stream: a tensor of another device must not reach it."""
+    require_cuda(*tensors)
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise RuntimeError(f"a tensor on {t.device} was passed while cuda:{cur} is the current device")
+
+
+def _bhsd(t, name, shape, dtype, *, written=False):
+    """(batch, head, row) strides of a [B, heads, rows, hd] view with unit inner stride; an axis of one element counts as 0."""
+    _need(t.dim() == 4 and tuple(t.shape) == tuple(shape) and t.dtype == dtype, f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
+    _need(t.stride(3) == 1, f"{name} needs unit stride along its last axis")
+    if written:
+        _need(all(t.stride(i) > 0 or t.shape[i] == 1 for i in range(3)), f"{name} is written: its rows must not overlap")
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3))
+
+
+def _lens_ptr(lens, B):
+    if lens is not None:
+        _need(lens.dtype == torch.int32 and tuple(lens.shape) == (B,) and lens.is_contiguous(), f"lens must be a contiguous int32 [{B}] tensor")
+    return ptr(lens)
+
+
+def _ws(workspace):
+    if workspace is None:
+        return None, 0
+    _need(workspace.is_contiguous(), "workspace must be contiguous")
+    return ptr(workspace), workspace.numel() * workspace.element_size()
+
+
+def attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> int:
+    """Bytes that let attn_window_fwd cut a call of few rows over many keys along the keys (0: it would not)."""
+    return _lib.load().capdec_attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
+
+
+def _fill_window(desc, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, *, o_written):
+    _on_current_device(q, k, v, o, lens, lse, workspace)
+    _need(q.dim() == 4 and k.dim() == 4, "q must be [B, H, nq, hd] and k [B, Hkv, S, hd]")
+    B, H, nq, hd = q.shape
+    Hkv, S = k.shape[1], k.shape[2]
+    desc.q, desc.k, desc.v, desc.o = ptr(q), ptr(k), ptr(v), ptr(o)
+    desc.q_bs, desc.q_hs, desc.q_ss = _bhsd(q, "q", (B, H, nq, hd), q.dtype)
+    desc.k_bs, desc.k_hs, desc.k_ss = _bhsd(k, "k", (B, Hkv, S, hd), q.dtype)
+    desc.v_bs, desc.v_hs, desc.v_ss = _bhsd(v, "v", (B, Hkv, S, hd), q.dtype)
+    desc.o_bs, desc.o_hs, desc.o_ss = _bhsd(o, "o", (B, H, nq, hd), q.dtype, written=o_written)
+    if lse is not None:
+        _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, nq) and lse.is_contiguous(), f"lse must be a contiguous float32 {[B, H, nq]} tensor")
+    desc.dtype = dtype_code(q)
+    desc.B, desc.H, desc.Hkv, desc.S, desc.hd = B, H, Hkv, S, hd
+    desc.q_start, desc.nq = q_start, nq
+    desc.window, desc.prefix_len, desc.prefix_open = window, prefix_len, int(prefix_open)
+    desc.lens = _lens_ptr(lens, B)
+    desc.drop = drop
+    desc.lse = ptr(lse)
+    desc.workspace, desc.workspace_bytes = _ws(workspace)
+
+
+def attn_window_fwd(q, k, v, o, *, window, prefix_len=0, prefix_open=False, q_start=0, lens=None, drop: Dropout = NO_DROPOUT, lse=None,
+                    workspace=None):
+    """Attention under a sliding window whose first prefix_len keys stay visible: q, o [B, H, nq, hd] (q pre-scaled, row r at
+    position q_start + r), k, v [B, Hkv, S, hd], any strides along the first three axes.  window counts the query's own key
+    (0: no limit); prefix_open lets queries before the prefix's end see all of it.  lens [B] int32: rows of each sequence;
+    lse [B, H, nq] f32 (optional) for the backward.  A query at or past its sequence's end gives 0 and lse -inf."""
+    desc = AttnWindowDesc()
+    _fill_window(desc, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written=True)
+    if q.numel() == 0:
+        return o
+    check(_lib.load().capdec_attn_window_fwd(C.byref(desc), _st()), "capdec_attn_window_fwd")
+    return o
+
+
+def attn_window_bwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> int:
+    return _lib.load().capdec_attn_window_bwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
+
+
+def attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, delta, *, window, prefix_len=0, prefix_open=False, q_start=0, lens=None,
+                    drop: Dropout = NO_DROPOUT, dq_scale=1.0, workspace=None):
+    """Gradients of attn_window_fwd (o and lse as it wrote them): dq [B, H, nq, hd], dk / dv [B, Hkv, S, hd], every row
+    written; delta [B, H, nq] f32 scratch.  workspace: attn_window_bwd_workspace bytes (allocated here if None)."""
+    desc = AttnWindowBwdDesc()
+    if workspace is None and q.dim() == 4 and k.dim() == 4 and q.is_cuda:
+        B, H, nq, hd = q.shape
+        workspace = torch.empty(attn_window_bwd_workspace(B, H, k.shape[1], k.shape[2], nq, hd, window=window, prefix_len=prefix_len),
+                                dtype=torch.uint8, device=q.device)
+    _need(lse is not None, "the backward needs the forward's lse")
+    _fill_window(desc.fwd, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written=False)
+    _on_current_device(dout, dq, dk, dv, delta)
+    B, H, nq, hd = q.shape
+    Hkv, S = k.shape[1], k.shape[2]
+    desc.dout, (desc.do_bs, desc.do_hs, desc.do_ss) = ptr(dout), _bhsd(dout, "dout", (B, H, nq, hd), q.dtype)
+    desc.dq, (desc.dq_bs, desc.dq_hs, desc.dq_ss) = ptr(dq), _bhsd(dq, "dq", (B, H, nq, hd), q.dtype, written=True)
+    desc.dk, (desc.dk_bs, desc.dk_hs, desc.dk_ss) = ptr(dk), _bhsd(dk, "dk", (B, Hkv, S, hd), q.dtype, written=True)
+    desc.dv, (desc.dv_bs, desc.dv_hs, desc.dv_ss) = ptr(dv), _bhsd(dv, "dv", (B, Hkv, S, hd), q.dtype, written=True)
+    _need(delta.dtype == torch.float32 and delta.numel() == B * H * nq and delta.is_contiguous(), "delta must be contiguous float32 scratch of B * H * nq")
+    desc.dq_scale = dq_scale
+    desc.delta = ptr(delta)
+    if q.numel() == 0:                      # no queries: nothing reaches a key
+        dk.zero_()
+        dv.zero_()
+        return
+    check(_lib.load().capdec_attn_window_bwd(C.byref(desc), _st()), "capdec_attn_window_bwd")
+
+
+def attn_window_decode_workspace(B, H, Hkv, hd, smax, *, window, prefix_len=0) -> int:
+    return _lib.load().capdec_attn_window_decode_workspace(B, H, Hkv, hd, smax, window, prefix_len)
+
+
+def attn_window_decode(q, kv_cache, o, *, window, prefix_len=0, length=None, lens=None, workspace=None):
+    """One query per sequence, its last position, over kv_cache [B, Hkv, 2, smax, hd]: q, o [B, H, hd] (or [B, H * hd]).
+    length: rows of every sequence (default smax); lens [B] int32 (optional): of each, at most length."""
+    _on_current_device(q, kv_cache, o, lens, workspace)
+    _need(kv_cache.dim() == 5 and kv_cache.shape[2] == 2 and kv_cache.is_contiguous(), "kv_cache must be a contiguous [B, Hkv, 2, smax, hd] tensor")
+    B, Hkv, _, smax, hd = kv_cache.shape
+    H = _decode_heads(q, o, B, hd)
+    _need(kv_cache.dtype == q.dtype, "q and kv_cache must have one dtype")
+    if q.numel() == 0:
+        return o
+    wp, wb = _ws(workspace)
+    check(_lib.load().capdec_attn_window_decode(ptr(q), ptr(kv_cache), ptr(o), dtype_code(q), B, H, Hkv, hd, smax, smax if length is None else length,
+                                                _lens_ptr(lens, B), window, prefix_len, wp, wb, _st()), "capdec_attn_window_decode")
+    return o
+
+
+def _decode_heads(q, o, B, hd):
+    _need(q.is_contiguous() and o.is_contiguous() and q.shape == o.shape and q.dtype == o.dtype, "q and o must be contiguous, of one shape and dtype")
+    _need(q.dim() in (2, 3) and q.shape[0] == B and q[0:1].numel() % hd == 0 and (q.dim() == 2 or q.shape[2] == hd), f"q must be [{B}, H, {hd}] or [{B}, H * {hd}]")
+    return q.shape[1] if q.dim() == 3 else q.shape[1] // hd
 
 
 def logits_ce_workspace(M, V) -> int:

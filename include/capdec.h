@@ -233,6 +233,61 @@ void capdec_attn_bwd_colsum_rows(int B, int S, int nq, int hd, long* q_rows, lon
 int capdec_attn_decode(const void* q, const void* kv_cache, void* o, int dtype,
                        int B, int H, int hd, int smax, int len, void* stream);
 
+/* ------------------------------------------------------------------ attention under a sliding window
+ * No reference counterpart.  Key j is visible to the query at position i of a sequence of n rows (i, j < n) when
+ *   j <= i and (j < prefix_len or window == 0 or i - j < window),
+ * and with prefix_open also whenever j < prefix_len: the first prefix_len keys (an image prefix, a few first tokens) stay
+ * visible however far the window has moved; window counts the query's own key, 0 means no limit.  A query that sees
+ * nothing -- one at or past its sequence's end -- gives zeros and lse -inf, and no gradient.
+ * q/o [B,H,nq,hd] (row r of q is position q_start + r), k/v [B,Hkv,S,hd], all addressed as base + b*bs + h*hs + s*ss + j
+ * (elements; rows 16-byte aligned, strides non-negative multiples of 16 bytes); q carries the hd^-0.5 scale.  Hkv divides H:
+ * query head h reads K/V head h / (H / Hkv).  hd 32, 64, 96 or 128; S < 2^28; q_start + nq <= S.
+ * lens [B] int32 on the DEVICE (NULL: every sequence has S rows): n of each sequence, taken into 0..S; K, V and q rows at or
+ * past n are never used, whatever they hold.  A non-finite value in a row that IS visible to some query of a call may
+ * reach other queries of its sequence.
+ * lse [B*H*nq] f32 (NULL: not wanted) receives the log-sum-exp the backward needs.
+ * workspace: with capdec_attn_window_fwd_workspace(...) bytes (0: none needed) a call of few rows over many keys is cut along
+ * the keys; NULL runs it in one piece.  Results do not depend on its contents; calls that overlap in time need their own. */
+typedef struct {
+    const void* q; const void* k; const void* v; void* o;
+    long q_bs, q_hs, q_ss;  long k_bs, k_hs, k_ss;  long v_bs, v_hs, v_ss;  long o_bs, o_hs, o_ss;
+    int dtype;
+    int B, H, Hkv, S, hd;
+    int q_start, nq;
+    int window, prefix_len, prefix_open;
+    const int32_t* lens;
+    capdec_dropout drop;     /* on probabilities; index ((b*H+h)*S+position)*S4+key, S4 = S rounded up to a multiple of 4 */
+    float* lse;
+    void* workspace; long workspace_bytes;
+} capdec_attn_window_desc;
+
+long capdec_attn_window_fwd_workspace(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix_len);
+int capdec_attn_window_fwd(const capdec_attn_window_desc* desc, void* stream);
+
+/* Backward: fwd as in the forward call (o and lse as it wrote them); dout/dq [B,H,nq,hd], dk/dv [B,Hkv,S,hd] (the sum over
+ * the heads that share a K/V head).  Every row of dq, dk and dv is written, zeros where nothing was visible.
+ * delta [B*H*nq] f32 scratch.  fwd.workspace: capdec_attn_window_bwd_workspace(...) bytes, required unless that is 0.
+ * No atomics: the same call gives the same bits. */
+typedef struct {
+    capdec_attn_window_desc fwd;
+    const void* dout; long do_bs, do_hs, do_ss;
+    void* dq; long dq_bs, dq_hs, dq_ss;
+    void* dk; long dk_bs, dk_hs, dk_ss;
+    void* dv; long dv_bs, dv_hs, dv_ss;
+    float dq_scale;          /* dq is multiplied by this (hd^-0.5 when q was pre-scaled) */
+    float* delta;
+} capdec_attn_window_bwd_desc;
+
+long capdec_attn_window_bwd_workspace(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix_len);
+int capdec_attn_window_bwd(const capdec_attn_window_bwd_desc* desc, void* stream);
+
+/* One query per sequence, its last position (len - 1), against a K/V cache [B][Hkv][2][smax][hd]: q, o [B, H*hd].  lens
+ * [B] int32 on the device (NULL: every sequence has len rows), taken into 0..len; a sequence of no rows gives zeros.
+ * workspace as above (capdec_attn_window_decode_workspace bytes fit every len <= smax). */
+long capdec_attn_window_decode_workspace(int B, int H, int Hkv, int hd, int smax, int window, int prefix_len);
+int capdec_attn_window_decode(const void* q, const void* kv_cache, void* o, int dtype, int B, int H, int Hkv, int hd, int smax, int len,
+                              const int32_t* lens, int window, int prefix_len, void* workspace, long workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ vocabulary projection + cross-entropy
  * Replaces decoder.py:66 (output_projection) on the scored rows only, the
  * slice/permute/reshape of decoder.py:172-179, nn.CrossEntropyLoss() (mean over
