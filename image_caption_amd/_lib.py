@@ -115,6 +115,15 @@ class AttnWindowBwdDesc(C.Structure):
     ]
 
 
+class Kv4Rows(C.Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p),
+        ("k_bs", c_long), ("k_hs", c_long), ("k_ss", c_long),
+        ("v_bs", c_long), ("v_hs", c_long), ("v_ss", c_long),
+        ("dtype", c_int), ("n", c_int),
+    ]
+
+
 class BlockParams(C.Structure):
     _fields_ = [(n, c_void_p) for n in (
         "norm1_w", "norm1_b", "in_proj_w", "in_proj_b", "out_proj_w", "out_proj_b", "norm2_w", "norm2_b",
@@ -179,6 +188,11 @@ SIGNATURES = {
     "capdec_attn_window_bwd": (c_int, [C.POINTER(AttnWindowBwdDesc), c_void_p]),
     "capdec_attn_window_decode_workspace": (c_long, [c_int] * 7),
     "capdec_attn_window_decode": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p, c_int, c_int, c_void_p, c_long, c_void_p]),
+    "capdec_kv4_head_bytes": (c_long, [c_int, c_int]),
+    "capdec_kv4_append": (c_int, [C.POINTER(Kv4Rows), c_void_p] + [c_int] * 5 + [c_void_p, c_void_p, c_void_p]),
+    "capdec_kv4_unpack": (c_int, [c_void_p, C.POINTER(Kv4Rows)] + [c_int] * 5 + [c_void_p, c_void_p]),
+    "capdec_attn_decode_kv4_workspace": (c_long, [c_int] * 7),
+    "capdec_attn_decode_kv4": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p, c_int, c_int, c_void_p, c_long, c_void_p]),
     "capdec_logits_ce_workspace": (c_long, [c_long, c_int]),
     "capdec_logits_ce_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_long, c_long,
                                      c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -422,6 +422,78 @@ def _decode_heads(q, o, B, hd):
     return q.shape[1] if q.dim() == 3 else q.shape[1] // hd
 
 
+def kv4_cache(B, Hkv, smax, hd, device) -> torch.Tensor:
+    """An empty cache of smax rows per sequence in 4 bits per value: [B, Hkv, bytes] uint8 (the layout is the library's own)."""
+    size = _lib.load().capdec_kv4_head_bytes(smax, hd)
+    _need(size > 0, f"no 4-bit cache of {smax} rows of {hd} channels (32, 64, 96 or 128)")
+    return torch.zeros(B, Hkv, size, dtype=torch.uint8, device=device)
+
+
+def _kv4_geometry(cache, smax, hd):
+    _need(cache.dim() == 3 and cache.dtype == torch.uint8 and cache.is_contiguous() and
+          cache.shape[2] == _lib.load().capdec_kv4_head_bytes(smax, hd) > 0, f"cache must come from kv4_cache(B, Hkv, {smax}, {hd}, device)")
+    return cache.shape[0], cache.shape[1]
+
+
+def _kv4_rows(k, v, B, Hkv, *, written=False):
+    t = k if k is not None else v
+    _need(t is not None and t.dim() == 4, "k and v must be [B, Hkv, n, hd]")
+    shape = (B, Hkv, t.shape[2], t.shape[3])
+    r = _lib.Kv4Rows()
+    if k is not None:
+        r.k, (r.k_bs, r.k_hs, r.k_ss) = ptr(k), _bhsd(k, "k", shape, t.dtype, written=written)
+    if v is not None:
+        r.v, (r.v_bs, r.v_hs, r.v_ss) = ptr(v), _bhsd(v, "v", shape, t.dtype, written=written)
+    r.dtype, r.n = dtype_code(t), t.shape[2]
+    return r
+
+
+def kv4_append(k, v, cache, *, smax, start=0, starts=None, counts=None):
+    """Quantises the rows k, v [B, Hkv, n, hd] into rows start.. (or starts[b]..) of a kv4_cache; counts[b] (optional): how many
+    of the n rows sequence b has.  With starts, rows that would fall outside the cache are dropped."""
+    _on_current_device(k, v, cache, starts, counts)
+    _need(k.dim() == 4, "k and v must be [B, Hkv, n, hd]")
+    B, Hkv = _kv4_geometry(cache, smax, k.shape[3])
+    rows = _kv4_rows(k, v, B, Hkv)
+    sp, cp = _lens_ptr(starts, B), _lens_ptr(counts, B)
+    if k.numel() == 0:
+        return cache
+    check(_lib.load().capdec_kv4_append(C.byref(rows), ptr(cache), B, Hkv, smax, k.shape[3], start, sp, cp, _st()), "capdec_kv4_append")
+    return cache
+
+
+def kv4_unpack(cache, k_out, v_out, *, smax, start=0, starts=None):
+    """The values that rows start.. (or starts[b]..) of a kv4_cache stand for, into k_out / v_out [B, Hkv, n, hd] (one may be None)."""
+    _on_current_device(cache, k_out, v_out, starts)
+    t = k_out if k_out is not None else v_out
+    _need(t is not None and t.dim() == 4, "k_out and v_out must be [B, Hkv, n, hd]")
+    B, Hkv = _kv4_geometry(cache, smax, t.shape[3])
+    rows = _kv4_rows(k_out, v_out, B, Hkv, written=True)
+    sp = _lens_ptr(starts, B)
+    if t.numel() == 0:
+        return
+    check(_lib.load().capdec_kv4_unpack(ptr(cache), C.byref(rows), B, Hkv, smax, t.shape[3], start, sp, _st()), "capdec_kv4_unpack")
+
+
+def attn_decode_kv4_workspace(B, H, Hkv, hd, smax, *, window=0, prefix_len=0) -> int:
+    return _lib.load().capdec_attn_decode_kv4_workspace(B, H, Hkv, hd, smax, window, prefix_len)
+
+
+def attn_decode_kv4(q, cache, o, *, smax, window=0, prefix_len=0, length=None, lens=None, workspace=None):
+    """attn_window_decode over a kv4_cache: q, o [B, H, hd]; every key is visible unless a window is given."""
+    _on_current_device(q, cache, o, lens, workspace)
+    _need(q.dim() == 3, "q must be [B, H, hd]")
+    hd = q.shape[2]
+    B, Hkv = _kv4_geometry(cache, smax, hd)
+    H = _decode_heads(q, o, B, hd)
+    if q.numel() == 0:
+        return o
+    wp, wb = _ws(workspace)
+    check(_lib.load().capdec_attn_decode_kv4(ptr(q), ptr(cache), ptr(o), dtype_code(q), B, H, Hkv, hd, smax, smax if length is None else length,
+                                             _lens_ptr(lens, B), window, prefix_len, wp, wb, _st()), "capdec_attn_decode_kv4")
+    return o
+
+
 def logits_ce_workspace(M, V) -> int:
     return _lib.load().capdec_logits_ce_workspace(M, V)
 

@@ -288,6 +288,38 @@ long capdec_attn_window_decode_workspace(int B, int H, int Hkv, int hd, int smax
 int capdec_attn_window_decode(const void* q, const void* kv_cache, void* o, int dtype, int B, int H, int Hkv, int hd, int smax, int len,
                               const int32_t* lens, int window, int prefix_len, void* workspace, long workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ K/V cache in 4 bits per value
+ * No reference counterpart.  A row of hd channels is cut into groups of 32; a group stands for offset + scale * level with
+ * levels 0..15 and, in f32 steps, offset = bf16(min), scale = bf16((max - min) * f32(1/15)), level = clamp(rint((x - offset) *
+ * (1 / scale)), 0, 15) (0 where the scale is 0).  A group that holds a NaN or an infinity stands for unspecified values.
+ * The layout is the library's own: one piece of capdec_kv4_head_bytes(smax, hd) bytes per (sequence, K/V head), [B][Hkv]
+ * pieces, 16-byte aligned; hd 32, 64, 96 or 128, smax < 2^28. */
+long capdec_kv4_head_bytes(int smax, int hd);
+
+/* n rows per sequence, k/v [B,Hkv,n,hd] of dtype addressed as base + b*bs + h*hs + s*ss + j (elements).  For
+ * capdec_kv4_unpack they are written, and one of k / v may be NULL. */
+typedef struct {
+    const void* k; const void* v;
+    long k_bs, k_hs, k_ss;  long v_bs, v_hs, v_ss;
+    int dtype, n;
+} capdec_kv4_rows;
+
+/* Quantises n new rows of every sequence into rows start.. of the cache (rows 16-byte aligned, strides multiples of 16
+ * bytes).  starts [B] int32 on the device (NULL: `start` for all): where each sequence's rows go; rows that would fall outside
+ * 0..smax-1 are dropped.  counts [B] int32 on the device (NULL: n for all): how many of the n rows each sequence has, taken
+ * into 0..n.  Other rows of the cache keep what they hold.  Two calls that may overlap in time must not write the same
+ * 32-row block of a sequence. */
+int capdec_kv4_append(const capdec_kv4_rows* rows, void* cache, int B, int Hkv, int smax, int hd, int start, const int32_t* starts,
+                      const int32_t* counts, void* stream);
+/* The values that rows start.. of the cache stand for (rows outside 0..smax-1 are not written). */
+int capdec_kv4_unpack(const void* cache, const capdec_kv4_rows* rows, int B, int Hkv, int smax, int hd, int start, const int32_t* starts,
+                      void* stream);
+/* capdec_attn_window_decode over such a cache (same visibility, lengths and workspace rules; window 0: every key).  bf16
+ * calls round the probabilities times their group's scale to bf16 once; f32 calls keep them. */
+long capdec_attn_decode_kv4_workspace(int B, int H, int Hkv, int hd, int smax, int window, int prefix_len);
+int capdec_attn_decode_kv4(const void* q, const void* cache, void* o, int dtype, int B, int H, int Hkv, int hd, int smax, int len,
+                           const int32_t* lens, int window, int prefix_len, void* workspace, long workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ vocabulary projection + cross-entropy
  * Replaces decoder.py:66 (output_projection) on the scored rows only, the
  * slice/permute/reshape of decoder.py:172-179, nn.CrossEntropyLoss() (mean over
