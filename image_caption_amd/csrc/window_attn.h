@@ -85,6 +85,12 @@ template <int HD> struct RowFrag<bf16_t, HD> {
 #pragma unroll
         for (int s = 0; s < HD / 16; ++s) f[s] = __builtin_bit_cast(bf16x8, (u32x4{0, 0, 0, 0}));
     }
+    // the loads have landed here: left to itself the compiler may sink them to a loop's first use, where their wait would be
+    // a wait for every later load as well, in every pass
+    __device__ __forceinline__ void landed() {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) asm volatile("" : "+v"(f[s]));
+    }
     // sum over this lane's half of the row
     __device__ __forceinline__ float dot(const RowFrag& o) const {
         float a = 0.f;
@@ -104,6 +110,10 @@ template <int HD> struct RowFrag<float, HD> {
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int s = 0; s < HD / 8; ++s) f[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void landed() {
+#pragma unroll
+        for (int s = 0; s < HD / 8; ++s) asm volatile("" : "+v"(f[s]));
     }
     __device__ __forceinline__ float dot(const RowFrag& o) const {
         float a = 0.f;
@@ -131,7 +141,25 @@ template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const ch
     }
 }
 
-// p is rounded to bf16 (half a step, 2^-9 of each term) to be an operand: the products' own inputs have no more bits
+// the same with the second operand's rows in LDS as well
+template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, bf16_t, int lane) {
+    const int at = (lane & 31) * WinGeo<bf16_t, HD>::PB + (lane >> 5) * 16;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(lds + at + 32 * s), *reinterpret_cast<const bf16x8*>(rows + at + 32 * s),
+                                                      acc, 0, 0, 0);
+}
+template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, float, int lane) {
+    const int at = (lane & 31) * WinGeo<float, HD>::PB + (lane >> 5) * 16;
+#pragma unroll
+    for (int s = 0; s < HD / 8; ++s) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at + 32 * s), b = *reinterpret_cast<const f32x4*>(rows + at + 32 * s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+    }
+}
+
+// p is rounded to bf16 (half a step, 2^-8 of each term) to be an operand: the products' own inputs have no more bits
 template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, bf16_t, int lane) {
     constexpr int PB = WinGeo<bf16_t, HD>::PB;
     const int g = lane >> 4, i = lane & 15;

@@ -25,6 +25,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     constexpr int NSUB = KW == 1 && sizeof(T) == 2 ? 2 : 1;
     constexpr int NT = 64 * QW * KW, BK = 32 * KW * NSUB, NBUF = KW == 1 ? 2 : 1;
     constexpr int MAT = BK * G::PB;
+    constexpr bool PRE = KW == 1 || HD < 128;          // the next tile's loads go out before this one's products, where the registers hold them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
@@ -132,9 +133,10 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
             for (int idx = 0; idx < tl.nt; ++idx) {
                 tp.commit(smem, smem + MAT, tid);
                 __syncthreads();
-                if (idx + 1 < tl.nt) fetch(idx + 1);
+                if (PRE && idx + 1 < tl.nt) fetch(idx + 1);
                 compute(idx, smem, smem + MAT);
                 __syncthreads();
+                if (!PRE && idx + 1 < tl.nt) fetch(idx + 1);
             }
         }
     }
@@ -207,62 +209,73 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
     const RowBlocks rb = win_row_blocks(p, k0, n);
     const int b_begin = rb.first + (int)((long)rb.count * chunk / nc), b_end = rb.first + (int)((long)rb.count * (chunk + 1) / nc);
 
-    RowFrag<T, HD> kf, vf;
-    kf.zero();
+    // K's rows stay in LDS and V's in registers: with both in registers the accumulators no longer fit beside them
+    char* lk = smem + 2 * BUF;
+    RowFrag<T, HD> vf;
     vf.zero();
-    if (key < n) {
-        kf.load(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)key * p.k_ss, lane);
-        vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+    {
+        u32x4 z[KT * CPR / 256];
+#pragma unroll
+        for (int j = 0; j < KT * CPR / 256; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            z[j] = u32x4{0, 0, 0, 0};
+            if (k0 + row < n)
+                z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)(k0 + row) * p.k_ss + ch * (16 / (int)sizeof(T)));
+        }
+        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+#pragma unroll
+        for (int j = 0; j < KT * CPR / 256; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            *reinterpret_cast<u32x4*>(lk + row * G::PB + ch * 16) = z[j];
+        }
     }
+    vf.landed();
+    const char* lkw = lk + 32 * wave * G::PB;
     f32x16 dk[G::DT], dv[G::DT];
 #pragma unroll
     for (int d = 0; d < G::DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
 
+    // the next block's rows on their way: loaded whatever they hold (rows past the end repeat the last one), and what may not
+    // be used -- rows at or past the sequence's end -- put to zero when they reach LDS, so that nothing here waits for a load
     u32x4 fq[U], fd[U];
-    float f_lse = INFINITY, f_delta = 0.f;
-    int f_pos = 0;
+    float f_lse = 0.f, f_delta = 0.f;
+    const T* qb = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)(hkv * p.G) * p.q_hs;
+    const T* db = reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)(hkv * p.G) * p.do_hs;
+    const long stat0 = ((long)b * p.H + hkv * p.G) * p.nq;
     auto fetch = [&](int blk) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR, r = blk * RB + row;
-            fq[j] = fd[j] = u32x4{0, 0, 0, 0};
-            if (row < RB && r < p.rows) {
-                const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
-                if (p.q_start + i < n) {
-                    fq[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i * p.q_ss + ch * (16 / (int)sizeof(T)));
-                    fd[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)h * p.do_hs + (long)i * p.do_ss + ch * (16 / (int)sizeof(T)));
-                }
-            }
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            const int r = min(blk * RB + row, p.rows - 1), i = win_row_query(p, r), g = r - i * p.G;
+            fq[j] = *reinterpret_cast<const u32x4*>(qb + (long)g * p.q_hs + (long)i * p.q_ss + ch * (16 / (int)sizeof(T)));
+            fd[j] = *reinterpret_cast<const u32x4*>(db + (long)g * p.do_hs + (long)i * p.do_ss + ch * (16 / (int)sizeof(T)));
         }
         if (tid < RB) {
-            const int r = blk * RB + tid, rc = min(r, p.rows - 1), i = win_row_query(p, rc), h = hkv * p.G + rc - i * p.G;
-            f_pos = p.q_start + i;
-            f_lse = INFINITY;                         // rows that are not there, and rows that see nothing: probability 0
-            f_delta = 0.f;
-            if (r < p.rows && f_pos < n) {
-                const long stat = ((long)b * p.H + h) * p.nq + i;
-                const float v = p.lse[stat];
-                f_lse = v == -INFINITY ? INFINITY : v;
-                f_delta = p.delta[stat];
-            }
+            const int r = min(blk * RB + tid, p.rows - 1), i = win_row_query(p, r), g = r - i * p.G;
+            f_lse = p.lse[stat0 + (long)g * p.nq + i];
+            f_delta = p.delta[stat0 + (long)g * p.nq + i];
         }
     };
-    auto commit = [&](char* buf) {
+    auto commit = [&](int blk, char* buf) {
+        // rows of a block are in the order of their positions: those before the sequence's end come first
+        const int live = min(p.rows, max(0, n - p.q_start) * p.G) - blk * RB;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
-            if (row < RB) {
-                *reinterpret_cast<u32x4*>(buf + row * G::PB + ch * 16) = fq[j];
-                *reinterpret_cast<u32x4*>(buf + MAT + row * G::PB + ch * 16) = fd[j];
+            if (RB * CPR % 256 == 0 || row < RB) {
+                const u32x4 z = {0, 0, 0, 0};
+                *reinterpret_cast<u32x4*>(buf + row * G::PB + ch * 16) = row < live ? fq[j] : z;
+                *reinterpret_cast<u32x4*>(buf + MAT + row * G::PB + ch * 16) = row < live ? fd[j] : z;
             }
         }
         if (tid < RB) {
             float* st = reinterpret_cast<float*>(buf + 2 * MAT);
-            st[tid] = f_lse;
-            st[RB + tid] = f_delta;
-            reinterpret_cast<int*>(st)[2 * RB + tid] = f_pos;
+            // rows that are not there, and rows that see nothing: probability 0.  (bf16: in units of the exponent of 2)
+            st[tid] = tid >= live || f_lse == -INFINITY ? INFINITY : (sizeof(T) == 2 ? f_lse * WIN_LOG2E : f_lse);
+            st[RB + tid] = tid >= live ? 0.f : f_delta;
+            reinterpret_cast<int*>(st)[2 * RB + tid] = p.q_start + win_row_query(p, min(blk * RB + tid, p.rows - 1));
         }
     };
     auto compute = [&](int blk, const char* buf) {
@@ -274,7 +287,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
         f32x16 s, dp;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-        mma_rows<HD>(s, buf, kf, lane);
+        mma_rows_lds<HD>(s, buf, lkw, T{}, lane);
         mma_rows<HD>(dp, buf + MAT, vf, lane);
         const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
         const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
             const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * jj);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = sizeof(T) == 2 ? fmaf(s[4 * jj + e], WIN_LOG2E, -lse[e] * WIN_LOG2E) : (s[4 * jj + e] - lse[e]) * WIN_LOG2E;
+                const float x = sizeof(T) == 2 ? fmaf(s[4 * jj + e], WIN_LOG2E, -lse[e]) : (s[4 * jj + e] - lse[e]) * WIN_LOG2E;
                 s[4 * jj + e] = __builtin_amdgcn_exp2f(x);
             }
         }
@@ -323,14 +336,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
     };
     if (b_begin < b_end) {
         fetch(b_begin);
-        commit(smem);
+        commit(b_begin, smem);
         __syncthreads();
         for (int blk = b_begin; blk < b_end; ++blk) {
             const int cur = (blk - b_begin) & 1;
             const bool more = blk + 1 < b_end;
             if (more) fetch(blk + 1);
             compute(blk, smem + cur * BUF);
-            if (more) commit(smem + (cur ^ 1) * BUF);
+            if (more) commit(blk + 1, smem + (cur ^ 1) * BUF);
             __syncthreads();
         }
     }
@@ -416,7 +429,7 @@ int bwd_go(WinArgs& a, hipStream_t st) {
     const long grid = bh * ((long)a.kp * a.ncp + (long)(a.ktiles - a.kp) * a.ncn);
     CAPDEC_CHECK(grid < (1L << 31), "attn_window_bwd: grid too large");
     auto kfn = win_dkv_kernel<T, HD, DROP>;
-    constexpr int lds = 2 * (2 * RB * G::PB + 3 * RB * 4);
+    constexpr int lds = 2 * (2 * RB * G::PB + 3 * RB * 4) + KT * G::PB;
     if (lds > 64 * 1024) ensure_dynamic_lds((const void*)kfn, lds);
     hipLaunchKernelGGL(kfn, dim3((unsigned)grid), dim3(256), lds, st, a);
     CAPDEC_LAUNCH_CHECK();

@@ -23,6 +23,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     using G = WinGeo<T, HD>;
     constexpr int NT = 64 * QW * KW, BK = 32 * KW * NSUB, NBUF = KW == 1 ? 2 : 1;
     constexpr int MAT = BK * G::PB;
+    constexpr bool PRE = KW == 1 || HD < 128;          // the next tile's loads go out before this one's products, where the registers hold them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
@@ -146,9 +147,10 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
             for (int idx = t_begin; idx < t_end; ++idx) {
                 tp.commit(smem, smem + MAT, tid);
                 __syncthreads();
-                if (idx + 1 < t_end) fetch(idx + 1);
+                if (PRE && idx + 1 < t_end) fetch(idx + 1);
                 compute(idx, smem, smem + MAT);
                 __syncthreads();
+                if (!PRE && idx + 1 < t_end) fetch(idx + 1);
             }
         }
     }
