@@ -826,8 +826,9 @@ class DecoderEngine:
         ops.gemm(dl, h, grads[HEAD_W], M=V, N=d, K=M, a_kmajor=True, b_kmajor=True)
         dx = self.buf("dx_all", (M, d), torch.float32, dev)
         ops.gemm(dl, W.head_w, dx, M=M, N=d, K=V, b_kmajor=True)
+        g2_done = False
         for i in reversed(range(geo.n_blocks)):
-            dx = self._block_bwd(i, W, grads, dx, B, S, dev, i > 0 or need_input_grad)
+            dx, g2_done = self._block_bwd(i, W, grads, dx, B, S, dev, i > 0 or need_input_grad, g2_done)
         self.input_grad = dx if need_input_grad else None
 
     # ------------------------------------------------------------------ KV-cached greedy decoding
