@@ -145,6 +145,10 @@ class DecodeDesc(C.Structure):
     ]
 
 
+class DecodeKv(C.Structure):
+    _fields_ = [("kv4", c_int), ("window", c_int), ("prefix_len", c_int)]
+
+
 class AdamPanels(C.Structure):
     _fields_ = [("panels", c_void_p), ("first", c_long), ("rows", c_long), ("K", c_int), ("panel_rows", c_long)]
 
@@ -225,6 +229,8 @@ SIGNATURES = {
     "capdec_greedy_update": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, C.c_int64, C.c_int64, c_void_p]),
     "capdec_decode_step_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
     "capdec_decode_step": (c_int, [C.POINTER(DecodeDesc), c_void_p]),
+    "capdec_decode_step_kv_workspace": (c_long, [c_int] * 7 + [C.POINTER(DecodeKv)]),
+    "capdec_decode_step_kv": (c_int, [C.POINTER(DecodeDesc), C.POINTER(DecodeKv), c_void_p]),
 }
 
 _lib = None

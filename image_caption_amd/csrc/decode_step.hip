@@ -15,9 +15,12 @@ struct StepBuffers {
     void* argmax_ws;
     long argmax_ws_bytes;
     long total;
+    // with a capdec_decode_kv: the new row's K and V before they are quantised, and the attention's split workspace
+    void *kvnew, *attn_ws;
+    long attn_ws_bytes, total_kv;
 };
 
-StepBuffers carve(char* base, int B, int d, int ff, int V, int dtype) {
+StepBuffers carve(char* base, int B, int d, int ff, int V, int dtype, int H = 0, int smax = 0, const capdec_decode_kv* kv = nullptr) {
     const long e = dtype == CAPDEC_BF16 ? 2 : 4;
     StepBuffers s;
     long off = 0;
@@ -36,6 +39,15 @@ StepBuffers carve(char* base, int B, int d, int ff, int V, int dtype) {
     s.argmax_ws = take(s.argmax_ws_bytes);
     s.hhp = take((long)B * d * e);
     s.total = off;
+    s.kvnew = s.attn_ws = nullptr;
+    s.attn_ws_bytes = 0;
+    if (kv) {
+        s.kvnew = kv->kv4 ? take(2L * B * d * e) : nullptr;
+        s.attn_ws_bytes = kv->kv4 ? capdec_attn_decode_kv4_workspace(B, H, H, d / H, smax, kv->window, kv->prefix_len)
+                                  : capdec_attn_window_decode_workspace(B, H, H, d / H, smax, kv->window, kv->prefix_len);
+        s.attn_ws = take(s.attn_ws_bytes);
+    }
+    s.total_kv = off;
     return s;
 }
 
@@ -64,7 +76,14 @@ extern "C" long capdec_decode_step_workspace(int B, int d_model, int dim_ff, int
     return carve(nullptr, B, d_model, dim_ff, vocab, dtype).total;
 }
 
-extern "C" int capdec_decode_step(const capdec_decode_desc* p, void* stream) {
+extern "C" long capdec_decode_step_kv_workspace(int B, int d_model, int nhead, int dim_ff, int vocab, int dtype, int smax, const capdec_decode_kv* kv) {
+    if (B <= 0 || d_model <= 0 || nhead <= 0 || d_model % nhead || dim_ff <= 0 || vocab <= 0 || smax <= 0) return 0;
+    return carve(nullptr, B, d_model, dim_ff, vocab, dtype, nhead, smax, kv).total_kv;
+}
+
+extern "C" int capdec_decode_step(const capdec_decode_desc* p, void* stream) { return capdec_decode_step_kv(p, nullptr, stream); }
+
+extern "C" int capdec_decode_step_kv(const capdec_decode_desc* p, const capdec_decode_kv* kv, void* stream) {
     CAPDEC_CHECK(p != nullptr, "decode_step: null descriptor");
     CAPDEC_CHECK(p->B > 0 && p->d_model > 0 && p->nhead > 0 && p->dim_ff > 0 && p->vocab > 0 && p->n_blocks > 0, "decode_step: bad geometry");
     CAPDEC_CHECK(p->d_model % p->nhead == 0, "decode_step: d_model not divisible by nhead");
@@ -74,13 +93,14 @@ extern "C" int capdec_decode_step(const capdec_decode_desc* p, void* stream) {
     const bool advance = p->t + 1 < p->max_len;
     CAPDEC_CHECK(!advance || (p->s_new > 0 && p->s_new < p->smax), "decode_step: appended row %d outside the cache (smax %d)", p->s_new, p->smax);
     const int B = p->B, d = p->d_model, ff = p->dim_ff, H = p->nhead, hd = d / H;
-    const long need = capdec_decode_step_workspace(B, d, ff, p->vocab, p->dtype);
+    CAPDEC_CHECK(!kv || (kv->window >= 0 && kv->prefix_len >= 0 && p->smax > 0), "decode_step: window %d, prefix %d", kv ? kv->window : 0, kv ? kv->prefix_len : 0);
+    const long need = kv ? capdec_decode_step_kv_workspace(B, d, H, ff, p->vocab, p->dtype, p->smax, kv) : capdec_decode_step_workspace(B, d, ff, p->vocab, p->dtype);
     if (!p->workspace || p->workspace_bytes < need) {
         capdec_set_error("decode_step: workspace %ld bytes < %ld", p->workspace_bytes, need);
         return CAPDEC_ERR_WORKSPACE;
     }
     CAPDEC_CHECK((((uintptr_t)p->workspace) & (ALIGN - 1)) == 0, "decode_step: workspace must be 256-byte aligned");
-    const StepBuffers s = carve((char*)p->workspace, B, d, ff, p->vocab, p->dtype);
+    const StepBuffers s = carve((char*)p->workspace, B, d, ff, p->vocab, p->dtype, H, p->smax, kv);
     const int cdt = p->dtype;
 
     // 1. score the newest row, pick the token, book-keep <eos>/<pad>
@@ -107,8 +127,23 @@ extern "C" int capdec_decode_step(const capdec_decode_desc* p, void* stream) {
         g.ldc = d;                                   // only the q columns reach C; K/V columns go to the cache
         g.col_scale = scale; g.col_scale_n = d;
         g.kv_cache = w.kv_cache; g.kv_q = d; g.kv_d = d; g.kv_B = B; g.kv_H = H; g.kv_hd = hd; g.kv_smax = p->smax; g.kv_s0 = p->s_new;
-        CAPDEC_TRY(capdec_gemm_bias_act(&g, stream));
-        CAPDEC_TRY(capdec_attn_decode(s.qs, w.kv_cache, s.os, cdt, B, H, hd, p->smax, p->s_new + 1, stream));
+        if (kv && kv->kv4) {
+            // the new row goes to a one-row [B][H][2][1][hd] cache first, and from there, quantised, to its place
+            g.kv_cache = s.kvnew; g.kv_smax = 1; g.kv_s0 = 0;
+            CAPDEC_TRY(capdec_gemm_bias_act(&g, stream));
+            const long e = cdt == CAPDEC_BF16 ? 2 : 4;
+            const capdec_kv4_rows row = {s.kvnew, (const char*)s.kvnew + hd * e, 2L * d, 2L * hd, hd, 2L * d, 2L * hd, hd, cdt, 1};
+            CAPDEC_TRY(capdec_kv4_append(&row, w.kv_cache, B, H, p->smax, hd, p->s_new, nullptr, nullptr, stream));
+            CAPDEC_TRY(capdec_attn_decode_kv4(s.qs, w.kv_cache, s.os, cdt, B, H, H, hd, p->smax, p->s_new + 1, nullptr, kv->window, kv->prefix_len,
+                                              s.attn_ws, s.attn_ws_bytes, stream));
+        } else {
+            CAPDEC_TRY(capdec_gemm_bias_act(&g, stream));
+            if (kv && kv->window > 0)
+                CAPDEC_TRY(capdec_attn_window_decode(s.qs, w.kv_cache, s.os, cdt, B, H, H, hd, p->smax, p->s_new + 1, nullptr, kv->window, kv->prefix_len,
+                                                     s.attn_ws, s.attn_ws_bytes, stream));
+            else
+                CAPDEC_TRY(capdec_attn_decode(s.qs, w.kv_cache, s.os, cdt, B, H, hd, p->smax, p->s_new + 1, stream));
+        }
         g = linear(s.os, w.out_proj_w, s.xm, B, d, d, cdt, CAPDEC_F32, w.out_proj_b);
         g.residual = xcur; g.ldr = d;
         CAPDEC_TRY(capdec_gemm_bias_act(&g, stream));

@@ -67,7 +67,7 @@ class TransformerDecoder(nn.Module):
         self._engine: Optional[DecoderEngine] = None
         self._shadow: Dict[str, tuple] = {}
         self._step = 0
-        self.prefix_len = 0          # needed by mask_mode="prefix_causal" when forward() gets a joined tensor
+        self.prefix_len = 0          # needed by the masks that keep a prefix visible when forward() gets a joined tensor
 
     # ------------------------------------------------------------------ plumbing
     @property
@@ -144,6 +144,11 @@ class TransformerDecoder(nn.Module):
             hidden = (cols >= 16 * 768) & (cols > rows)
         elif mode == "prefix_causal":
             hidden = (cols >= self.prefix_len) & (cols > rows)
+        elif mode in ("prefix_window", "window"):
+            near = cols > rows - self.options.window if self.options.window else torch.ones_like(cols > rows)
+            hidden = ~((cols <= rows) & ((cols < self.prefix_len) | near))
+            if mode == "prefix_window":
+                hidden = hidden & (cols >= self.prefix_len)
         else:
             hidden = torch.zeros(seq_len, seq_len, dtype=torch.bool, device=dev)
         return torch.zeros(seq_len, seq_len, device=dev).masked_fill(hidden, float("-inf"))

@@ -11,6 +11,7 @@ What each stage replaces in the reference:
   scored-row vocab + CE       decoder.py:66,172-185
   backward                    decoder.py:189 (autograd of the above)
   greedy decoding             no counterpart (the reference has no generation code)
+  window masks, 4-bit caches  no counterpart
 """
 from __future__ import annotations
 
@@ -42,6 +43,9 @@ MATRIX_KEYS = ("self_attn.in_proj_weight", "self_attn.out_proj.weight", "linear1
 HEAD_W, HEAD_B = "output_projection.weight", "output_projection.bias"
 
 _MASKS = {"none": MASK_NONE, "reference": MASK_REFERENCE, "prefix_causal": MASK_PREFIX_CAUSAL}
+# masks of attn_window_*: a window over the text, the image prefix visible throughout -- to every row ("prefix_window"), or
+# only to the rows after each of its own ("window")
+_WINDOW_MASKS = {"prefix_window": True, "window": False}
 _ACTS = {"relu": ACT_RELU, "gelu": ACT_GELU}
 
 
@@ -49,7 +53,9 @@ _ACTS = {"relu": ACT_RELU, "gelu": ACT_GELU}
 class EngineOptions:
     """Knobs that have no counterpart in the reference's config.py."""
     compute_dtype: torch.dtype = torch.bfloat16   # bfloat16 = MFMA path, float32 = exact validation path
-    mask_mode: str = "reference"                  # decoder.py:31-38 literally; "prefix_causal" / "none"
+    mask_mode: str = "reference"                  # decoder.py:31-38 literally; "prefix_causal" / "none" / "prefix_window" / "window"
+    window: int = 0                               # the window masks: how many last keys a row sees, its own among them (0: no limit)
+    kv_cache_bits: int = 0                        # greedy decoding: 4 = the K/V cache holds 4 bits per value; 0 = the compute dtype
     activation: str = "relu"                      # decoder.py:60; "gelu" is an extension
     vocab_slab: int = 0                           # vocabulary columns per backward slab; 0: as wide as dl_budget_bytes allows
     dl_budget_bytes: int = 16 << 30               # cap on the d(logits) slab buffer (the whole vocabulary fits up to batch 5000 per GPU)
@@ -248,8 +254,12 @@ class DecoderEngine:
         self.opt = options or EngineOptions()
         if geo.d_model % geo.nhead:
             raise ValueError("d_model must be divisible by nhead")
-        if self.opt.mask_mode not in _MASKS:
-            raise ValueError(f"mask_mode must be one of {sorted(_MASKS)}")
+        if self.opt.mask_mode not in _MASKS and self.opt.mask_mode not in _WINDOW_MASKS:
+            raise ValueError(f"mask_mode must be one of {sorted(_MASKS) + sorted(_WINDOW_MASKS)}")
+        if self.opt.window < 0 or (self.opt.window and self.opt.mask_mode not in _WINDOW_MASKS):
+            raise ValueError(f"window {self.opt.window} needs mask_mode 'prefix_window' or 'window'")
+        if self.opt.kv_cache_bits not in (0, 4):
+            raise ValueError("kv_cache_bits must be 0 (the compute dtype) or 4")
         if self.opt.activation not in _ACTS:
             raise ValueError(f"activation must be one of {sorted(_ACTS)}")
         _lib.load()
@@ -323,6 +333,31 @@ class DecoderEngine:
         p = self.geo.dropout if train else 0.0
         return ops.dropout_keys(self.opt.dropout_seed, site, step, p)
 
+    # ------------------------------------------------------------------ window masks
+    def _window_kw(self, prefix_len):
+        return dict(window=self.opt.window, prefix_len=prefix_len, prefix_open=_WINDOW_MASKS[self.opt.mask_mode])
+
+    def _head_views(self, packed, B, S, parts, q_start=0):
+        """[B, H, rows, hd] views of the parts (q, k, v or o) of a packed [S*B, parts*d] matrix; the first from q_start on."""
+        t = packed.view(S, B, parts, self.geo.nhead, self.geo.hd)
+        return [t[q_start if i == 0 else 0:, :, i].permute(1, 2, 0, 3) for i in range(parts)]
+
+    def _window_fwd(self, qkv, o, lse, B, S, q_start, drop, dev):
+        H, hd, nq = self.geo.nhead, self.geo.hd, S - q_start
+        q, k, v = self._head_views(qkv, B, S, 3, q_start)
+        ws = self.buf("win_ws", (ops.attn_window_fwd_workspace(B, H, H, S, nq, hd, window=self.opt.window, prefix_len=self.prefix_len),), torch.uint8, dev)
+        ops.attn_window_fwd(q, k, v, self._head_views(o, B, S, 1, q_start)[0], q_start=q_start, drop=drop, lse=lse[:B * H * nq].view(B, H, nq),
+                            workspace=ws, **self._window_kw(self.prefix_len))
+
+    def _window_bwd(self, qkv, o, lse, do, dqkv, delta, B, S, q_start, drop, dev):
+        H, hd, nq = self.geo.nhead, self.geo.hd, S - q_start
+        q, k, v = self._head_views(qkv, B, S, 3, q_start)
+        dq, dk, dv = self._head_views(dqkv, B, S, 3, q_start)
+        (ov,), (dov,) = self._head_views(o, B, S, 1, q_start), self._head_views(do, B, S, 1, q_start)
+        ws = self.buf("win_bwd_ws", (ops.attn_window_bwd_workspace(B, H, H, S, nq, hd, window=self.opt.window, prefix_len=self.prefix_len),), torch.uint8, dev)
+        ops.attn_window_bwd(q, k, v, ov, lse[:B * H * nq].view(B, H, nq), dov, dq, dk, dv, delta[:B * H * nq], q_start=q_start, drop=drop,
+                            dq_scale=hd ** -0.5, workspace=ws, **self._window_kw(self.prefix_len))
+
     # ------------------------------------------------------------------ one block, forward
     def _block_fwd(self, i, W, x_in, B, S, q_start, train, step, dev, h1_ready=None, in_proj=None):
         """x_in [S*B,d] f32 -> rows q_start*B.. of the block output [Mt,d] f32.  Saves
@@ -358,8 +393,11 @@ class DecoderEngine:
         lse = self.buf(f"lse.{i}", (B * H * S,), torch.float32, dev)
         k_attn = self._keys(4 * i + 0, step, train)
         with self._span("block_attn_fwd"):
-            ops.attn_fwd_packed(qkv, attn_o, lse, B, H, S, hd, q_start=q_start, nq=S - q_start,
-                                mask_mode=_MASKS[self.opt.mask_mode], prefix_len=self.prefix_len, drop=k_attn)
+            if self.opt.mask_mode in _WINDOW_MASKS:
+                self._window_fwd(qkv, attn_o, lse, B, S, q_start, k_attn, dev)
+            else:
+                ops.attn_fwd_packed(qkv, attn_o, lse, B, H, S, hd, q_start=q_start, nq=S - q_start,
+                                    mask_mode=_MASKS[self.opt.mask_mode], prefix_len=self.prefix_len, drop=k_attn)
         x_mid = self.buf(f"x_mid.{i}", (Mt, d), torch.float32, dev)
         k_r1 = self._keys(4 * i + 1, step, train)
         with self._span("block_out_proj_fwd"):
@@ -405,8 +443,8 @@ class DecoderEngine:
             _lib.require_cuda(tgt)
             S, B, _ = tgt.shape
             self.prefix_len = source[2] if len(source) > 2 else 0
-        if self.opt.mask_mode == "prefix_causal" and self.prefix_len <= 0 and source[0] != "concat":
-            raise ValueError("prefix_causal masking needs the prefix length")
+        if self.opt.mask_mode in ("prefix_causal", "prefix_window") and self.prefix_len <= 0 and source[0] != "concat":
+            raise ValueError(f"{self.opt.mask_mode} masking needs the prefix length")
         dev = source[1].device
         M = S * B
         self.generation += 1
@@ -687,8 +725,11 @@ class DecoderEngine:
         dqkv = self.buf("dqkv", (M, 3 * d), cdt, dev)
         delta = self.buf("delta", (B * H * S,), torch.float32, dev)
         with self._span("block_attn_bwd"):
-            ops.attn_bwd_packed(sv["qkv"], sv["attn_o"], sv["lse"], dattn, dqkv, delta, B, H, S, hd, q_start=q_start, nq=S - q_start,
-                                mask_mode=_MASKS[self.opt.mask_mode], prefix_len=self.prefix_len, drop=k_attn, dq_scale=hd ** -0.5)
+            if self.opt.mask_mode in _WINDOW_MASKS:
+                self._window_bwd(sv["qkv"], sv["attn_o"], sv["lse"], dattn, dqkv, delta, B, S, q_start, k_attn, dev)
+            else:
+                ops.attn_bwd_packed(sv["qkv"], sv["attn_o"], sv["lse"], dattn, dqkv, delta, B, H, S, hd, q_start=q_start, nq=S - q_start,
+                                    mask_mode=_MASKS[self.opt.mask_mode], prefix_len=self.prefix_len, drop=k_attn, dq_scale=hd ** -0.5)
         gin_w, gin_b = G("self_attn.in_proj_weight"), G("self_attn.in_proj_bias")
         h1 = sv["h1"]
         # in_proj's bias gradient = column sums of dQKV = dQKV^T . 1: one more column of its weight-gradient product, formed by
@@ -841,14 +882,17 @@ class DecoderEngine:
         geo, cdt = self.geo, self.cdt
         d, ff, H, hd, V, nb = geo.d_model, geo.dim_feedforward, geo.nhead, geo.hd, geo.vocab_size, geo.n_blocks
         _lib.require_cuda(img, sos_slot, emb)
-        if nb > 1 and self.opt.mask_mode != "prefix_causal":
-            raise ValueError("KV-cached decoding with stacked blocks is only exact under mask_mode='prefix_causal'")
+        windowed, four = self.opt.mask_mode in _WINDOW_MASKS, self.opt.kv_cache_bits == 4
+        if nb > 1 and self.opt.mask_mode != "prefix_causal" and not windowed:
+            raise ValueError("KV-cached decoding with stacked blocks is only exact under mask_mode='prefix_causal', 'prefix_window' or 'window'")
         B, P, _ = img.shape
         dev = img.device
         S0, smax = P + 2, P + 1 + max_len
-        mask = _MASKS[self.opt.mask_mode]
         scale = hd ** -0.5
-        caches = [self.buf(f"kv.{i}", (B, H, 2, smax, hd), cdt, dev) for i in range(nb)]
+        if four:
+            caches = [self.buf(f"kv4.{i}", (B, H, _lib.load().capdec_kv4_head_bytes(smax, hd)), torch.uint8, dev) for i in range(nb)]
+        else:
+            caches = [self.buf(f"kv.{i}", (B, H, 2, smax, hd), cdt, dev) for i in range(nb)]
         ids = torch.full((B,), sos_id, dtype=torch.int64, device=dev)
         first = self.buf("gen_first", (B, 1, d), torch.float32, dev)
         ops.embed_rows(emb, ids, first.view(B, d))
@@ -867,17 +911,37 @@ class DecoderEngine:
             r0 = q0 * B
             if i > 0:
                 ops.ln_fwd(x, w["norm1.weight"], w["norm1.bias"], h1)
-            q = self.buf("gen_q", (M0, d), cdt, dev)
-            # K/V of all rows straight into the cache; q rows only where needed
             in_w, in_b = w["self_attn.in_proj_weight"], w["self_attn.in_proj_bias"]
-            if q0 == 0:
-                ops.gemm(h1, in_w, q, bias=in_b, col_scale=scale, col_scale_n=d, kv_cache=caches[i], kv_geom=(d, d, B, H, hd, smax, 0))
-            else:
-                ops.gemm(h1, in_w[d:], q, bias=in_b[d:], kv_cache=caches[i], kv_geom=(0, d, B, H, hd, smax, 0))
-                ops.gemm(h1[r0:], in_w[:d], q[r0:], bias=in_b[:d], col_scale=scale, col_scale_n=d)
             o = self.buf("gen_o", (M0, d), cdt, dev)
-            desc_strides = ((d, hd, B * d), kvs, kvs, (d, hd, B * d))
-            self._attn_cache_fwd(q, caches[i], o, desc_strides, B, H, S0, hd, smax, q0, S0 - q0, mask, P)
+            if four:
+                # the prompt attends to its own K and V; what the cache keeps of them is quantised on the way in
+                qkv = self.buf("gen_qkv", (M0, 3 * d), cdt, dev)
+                if q0 == 0:
+                    ops.gemm(h1, in_w, qkv, bias=in_b, col_scale=scale, col_scale_n=d)
+                else:
+                    ops.gemm(h1, in_w[d:], qkv[:, d:], bias=in_b[d:])
+                    ops.gemm(h1[r0:], in_w[:d], qkv[r0:, :d], bias=in_b[:d], col_scale=scale, col_scale_n=d)
+                if windowed:
+                    q, k, v = self._head_views(qkv, B, S0, 3, q0)
+                    ops.attn_window_fwd(q, k, v, self._head_views(o, B, S0, 1, q0)[0], q_start=q0, **self._window_kw(P))
+                else:
+                    ops.attn_fwd_packed(qkv, o, None, B, H, S0, hd, q_start=q0, nq=S0 - q0, mask_mode=_MASKS[self.opt.mask_mode], prefix_len=P)
+                    _, k, v = self._head_views(qkv, B, S0, 3)
+                ops.kv4_append(k, v, caches[i], smax=smax)
+            else:
+                q = self.buf("gen_q", (M0, d), cdt, dev)
+                # K/V of all rows straight into the cache; q rows only where needed
+                if q0 == 0:
+                    ops.gemm(h1, in_w, q, bias=in_b, col_scale=scale, col_scale_n=d, kv_cache=caches[i], kv_geom=(d, d, B, H, hd, smax, 0))
+                else:
+                    ops.gemm(h1, in_w[d:], q, bias=in_b[d:], kv_cache=caches[i], kv_geom=(0, d, B, H, hd, smax, 0))
+                    ops.gemm(h1[r0:], in_w[:d], q[r0:], bias=in_b[:d], col_scale=scale, col_scale_n=d)
+                if windowed:
+                    ops.attn_window_fwd(self._head_views(q, B, S0, 1, q0)[0], caches[i][:, :, 0, :S0], caches[i][:, :, 1, :S0],
+                                        self._head_views(o, B, S0, 1, q0)[0], q_start=q0, **self._window_kw(P))
+                else:
+                    desc_strides = ((d, hd, B * d), kvs, kvs, (d, hd, B * d))
+                    self._attn_cache_fwd(q, caches[i], o, desc_strides, B, H, S0, hd, smax, q0, S0 - q0, _MASKS[self.opt.mask_mode], P)
             Mt = M0 - r0
             x_mid = self.buf("gen_xmid", (Mt, d), torch.float32, dev)
             ops.gemm(o[r0:], w["self_attn.out_proj.weight"], x_mid, bias=w["self_attn.out_proj.bias"], residual=x[r0:])
@@ -903,7 +967,7 @@ class DecoderEngine:
             # per-kernel event brackets are wanted: issue the step's launches one by one (the same kernels,
             # in the same order, as capdec_decode_step)
             self._decode_loop_by_op(W, caches, x_last, emb, pos, ids, done, out, margins, max_len, S0, smax, eos_id, pad_id,
-                                    stop_check_every, w_panels)
+                                    stop_check_every, w_panels, P)
             return (out, margins) if return_margins else out
         mg = self.buf("gen_margin", (B,), torch.float32, dev)
         # the residual stream of the newest row lives in one buffer that every step reads and rewrites
@@ -915,7 +979,9 @@ class DecoderEngine:
                 raise ValueError(f"pos has {pos.shape[0]} rows, decoding needs {smax}")
         import ctypes as C
         lib = _lib.load()
-        wsb = lib.capdec_decode_step_workspace(B, d, ff, V, _lib.dtype_code(caches[0]))
+        code = _lib.BF16 if cdt == torch.bfloat16 else _lib.F32
+        kv = _lib.DecodeKv(int(four), self.opt.window if windowed else 0, P) if four or windowed else None
+        wsb = lib.capdec_decode_step_workspace(B, d, ff, V, code) if kv is None else lib.capdec_decode_step_kv_workspace(B, d, H, ff, V, code, smax, kv)
         ws = self.buf("gen_step_ws", (wsb,), torch.uint8, dev)
         blocks = (_lib.BlockParams * nb)()
         for i in range(nb):
@@ -930,7 +996,7 @@ class DecoderEngine:
             blocks[i].kv_cache = caches[i].data_ptr()
         dd = _lib.DecodeDesc()
         dd.B, dd.d_model, dd.nhead, dd.dim_ff, dd.vocab, dd.n_blocks, dd.smax = B, d, H, ff, V, nb, smax
-        dd.dtype, dd.activation, dd.ln_eps = _lib.dtype_code(caches[0]), _ACTS[self.opt.activation], 1e-5
+        dd.dtype, dd.activation, dd.ln_eps = code, _ACTS[self.opt.activation], 1e-5
         dd.blocks = blocks
         dd.head_w, dd.head_b, dd.ld_head_w = W.head_w.data_ptr(), W.head_b.data_ptr(), W.head_w.stride(0)
         dd.emb, dd.pos = emb.data_ptr(), (pos.data_ptr() if pos is not None else None)
@@ -944,7 +1010,7 @@ class DecoderEngine:
         for t in range(max_len):
             dd.t, dd.s_new = t, S0 + t                               # s_new: index of the row appended after token t
             with self._span("decode_step"):
-                _lib.check(lib.capdec_decode_step(C.byref(dd), stream), "capdec_decode_step")
+                _lib.check(lib.capdec_decode_step_kv(C.byref(dd), kv, stream), "capdec_decode_step")
             if return_margins:
                 margins[:, t].copy_(mg)
             # <eos> early stop: the remaining columns already hold <pad>.  Looking at `done` is a host
@@ -954,11 +1020,16 @@ class DecoderEngine:
         return (out, margins) if return_margins else out
 
     def _decode_loop_by_op(self, W, caches, x_last, emb, pos, ids, done, out, margins, max_len, S0, smax, eos_id, pad_id,
-                           stop_check_every, w_panels=None):
+                           stop_check_every, w_panels=None, prefix_len=0):
         geo, cdt = self.geo, self.cdt
+        four, window = self.opt.kv_cache_bits == 4, self.opt.window if self.opt.mask_mode in _WINDOW_MASKS else 0
         d, ff, H, hd, V, nb = geo.d_model, geo.dim_feedforward, geo.nhead, geo.hd, geo.vocab_size, geo.n_blocks
         B, dev, scale = ids.shape[0], ids.device, geo.hd ** -0.5
         return_margins = margins is not None
+        if four or window:
+            size = ops.attn_decode_kv4_workspace if four else ops.attn_window_decode_workspace
+            aws = self.buf("gen_attn_ws", (size(B, H, H, hd, smax, window=window, prefix_len=prefix_len),), torch.uint8, dev)
+            kv_new = self.buf("gen_kv_new", (B, H, 2, 1, hd), cdt, dev)
         ws = self.buf("gen_ws", (ops.logits_ce_workspace(B, V),), torch.uint8, dev)
         hh = self.buf("gen_hh", (B, d), cdt, dev)
         mg = self.buf("gen_margin", (B,), torch.float32, dev)
@@ -994,9 +1065,17 @@ class DecoderEngine:
                 w = W.blocks[i]
                 ops.ln_fwd(xcur, w["norm1.weight"], w["norm1.bias"], hs)
                 ops.gemm(hs, w["self_attn.in_proj_weight"], qs, bias=w["self_attn.in_proj_bias"], col_scale=scale, col_scale_n=d,
-                         kv_cache=caches[i], kv_geom=(d, d, B, H, hd, smax, s_new))
+                         kv_cache=kv_new if four else caches[i], kv_geom=(d, d, B, H, hd, 1, 0) if four else (d, d, B, H, hd, smax, s_new))
+                if four:
+                    ops.kv4_append(kv_new[:, :, 0], kv_new[:, :, 1], caches[i], smax=smax, start=s_new)
                 with self._span("attn_decode"):
-                    ops.attn_decode(qs, caches[i], os_, B, H, hd, smax, s_new + 1)
+                    if four:
+                        ops.attn_decode_kv4(qs.view(B, H, hd), caches[i], os_.view(B, H, hd), smax=smax, window=window, prefix_len=prefix_len,
+                                            length=s_new + 1, workspace=aws)
+                    elif window:
+                        ops.attn_window_decode(qs, caches[i], os_, window=window, prefix_len=prefix_len, length=s_new + 1, workspace=aws)
+                    else:
+                        ops.attn_decode(qs, caches[i], os_, B, H, hd, smax, s_new + 1)
                 ops.gemm(os_, w["self_attn.out_proj.weight"], xm, bias=w["self_attn.out_proj.bias"], residual=xcur)
                 ops.ln_fwd(xm, w["norm2.weight"], w["norm2.bias"], h2s)
                 ops.gemm(h2s, w["linear1.weight"], a1s, bias=w["linear1.bias"], act=_ACTS[self.opt.activation])

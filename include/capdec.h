@@ -536,6 +536,17 @@ typedef struct {
 long capdec_decode_step_workspace(int B, int d_model, int dim_ff, int vocab, int dtype);
 int capdec_decode_step(const capdec_decode_desc* desc, void* stream);
 
+/* capdec_decode_step with another attention over the caches: a window (0: every key) with prefix_len first keys kept
+ * (capdec_attn_window_decode), and / or caches of 4 bits per value (kv4: every block's kv_cache is then a cache of
+ * capdec_kv4_head_bytes(smax, d_model / nhead) bytes per sequence and head, 16-byte aligned, rows 0..s_new-1 appended).
+ * kv NULL: capdec_decode_step itself.  workspace: capdec_decode_step_kv_workspace(...) bytes. */
+typedef struct {
+    int kv4, window, prefix_len;
+} capdec_decode_kv;
+
+long capdec_decode_step_kv_workspace(int B, int d_model, int nhead, int dim_ff, int vocab, int dtype, int smax, const capdec_decode_kv* kv);
+int capdec_decode_step_kv(const capdec_decode_desc* desc, const capdec_decode_kv* kv, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

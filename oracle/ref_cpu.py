@@ -68,6 +68,8 @@ def caption_mask(seq_len: int, mode: str = "reference", prefix_len: int = 0) -> 
     16*768 set to 0, then triu(diagonal=1).  For S <= 12288 this is all zeros.
     mode "prefix_causal" (build-defined): key j is visible to query i when
     j < prefix_len or j <= i.
+    mode "prefix_window:W" (build-defined): key j is visible when j < prefix_len or i - W < j <= i; "window:W": when j <= i and
+    (j < prefix_len or j > i - W).
     mode "none": zeros.
     """
     if mode == "reference":
@@ -81,6 +83,14 @@ def caption_mask(seq_len: int, mode: str = "reference", prefix_len: int = 0) -> 
         m = torch.zeros(seq_len, seq_len)
         m[~vis] = float("-inf")
         return m
+    if mode.startswith(("window:", "prefix_window:")):
+        kind, W = mode.split(":")
+        i = torch.arange(seq_len)[:, None]
+        j = torch.arange(seq_len)[None, :]
+        vis = (j <= i) & ((j < prefix_len) | (i - j < int(W)))
+        if kind == "prefix_window":
+            vis = vis | (j < prefix_len)
+        return torch.zeros(seq_len, seq_len).masked_fill(~vis, float("-inf"))
     if mode == "none":
         return torch.zeros(seq_len, seq_len)
     raise ValueError(f"unknown mask mode {mode!r}")

@@ -164,3 +164,24 @@ def test_struct_layouts_match_c(tmp_path):
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     W, WB = _lib.AttnWindowDesc, _lib.AttnWindowBwdDesc
     assert got == [ctypes.sizeof(W), W.lens.offset, W.workspace_bytes.offset, ctypes.sizeof(WB), WB.dout.offset, WB.delta.offset]
+
+
+@pytest.mark.parametrize("mode,window", [("prefix_window", 3), ("window", 3), ("prefix_window", 0), ("window", 0)])
+def test_model_mask_is_the_oracles(mode, window):
+    from image_caption_amd.decoder import TransformerDecoder
+    from image_caption_amd.engine import EngineOptions
+    from oracle import ref_cpu
+    m = TransformerDecoder(64, 2, 6, 128, 0.0, 503, options=EngineOptions(mask_mode=mode, window=window))
+    m.prefix_len = 4
+    see = wo.masks(1, 12, 12, 0, [12], window, 4, mode == "prefix_window", "cpu")[0]
+    assert torch.equal(m.create_caption_mask(12) == 0, see)
+    if window:
+        assert torch.equal(ref_cpu.caption_mask(12, f"{mode}:{window}", 4) == 0, see)
+
+
+def test_engine_options_refused():
+    from image_caption_amd.engine import DecoderEngine, EngineOptions, ModelGeometry
+    geo = ModelGeometry(64, 2, 128, 503)
+    for bad in (dict(mask_mode="windows"), dict(window=4), dict(mask_mode="prefix_window", window=-1), dict(kv_cache_bits=8)):
+        with pytest.raises(ValueError):
+            DecoderEngine(geo, EngineOptions(**bad))
