@@ -151,32 +151,45 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs p) {
 // ------------------------------------------------------------------ read rows back
 struct UnpackArgs {
     const char* cache; long smax, sm; int B, Hkv, n; int start; const int32_t* starts;
-    void* k; void* v; long k_bs, k_hs, k_ss, v_bs, v_hs, v_ss; int dtype;
+    void* k; void* v; long k_bs, k_hs, k_ss, v_bs, v_hs, v_ss;
 };
-template <int HD>
+// Four channels of K and of V per thread, neighbouring threads on neighbouring channels: whole lines leave.  A word of V holds
+// eight keys of one channel, so it is read for each of them; the 16-32 rows a workgroup works on share their words in its L1.
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_unpack_kernel(UnpackArgs p) {
     using G = K4<HD>;
     const int bh = blockIdx.x, b = bh / p.Hkv, h = bh - b * p.Hkv;
     const long start = p.starts ? p.starts[b] : p.start;
     const char* piece = p.cache + bh * k4_piece(p.sm, HD);
-    const long total = (long)p.n * HD / 8;                                   // eight channels of K and of V per thread
+    const long total = (long)p.n * (HD / 4);
     for (long u = (long)blockIdx.y * 256 + threadIdx.x; u < total; u += (long)gridDim.y * 256) {
-        const long src = u / (HD / 8), key = start + src;
+        const int src = (int)(u / (HD / 4)), c4 = (int)(u - (long)src * (HD / 4)) * 4;
+        const long key = start + src;
         if (key < 0 || key >= p.smax) continue;
-        const int c8 = (int)(u - src * (HD / 8)), t = c8 >> 2, g = c8 & 3;
-        const unsigned ks = *reinterpret_cast<const unsigned*>(piece + k4_ks(p.sm, HD) + (key * G::NG + t) * 4);
-        const unsigned vs = *reinterpret_cast<const unsigned*>(piece + k4_vs(p.sm, HD) + (key * G::NG + t) * 4);
-        const unsigned kw = *reinterpret_cast<const unsigned*>(piece + k4_k_word<HD>((int)key, t, g));
-        const int vg = (int)(key & 15) >> 2, vj = (int)(key & 3) + 4 * (int)((key >> 4) & 1);
-        const long ko = (long)b * p.k_bs + (long)h * p.k_hs + src * p.k_ss + 8 * c8, vo = (long)b * p.v_bs + (long)h * p.v_hs + src * p.v_ss + 8 * c8;
+        const int t = c4 >> 5, g = (c4 >> 3) & 3;
+        auto put = [&](void* base, long at, const float (&x)[4]) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(reinterpret_cast<T*>(base) + at) = bf16x4{(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3]};
+            else *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(base) + at) = f32x4{x[0], x[1], x[2], x[3]};
+        };
+        float x[4];
+        if (p.k) {
+            const unsigned sw = *reinterpret_cast<const unsigned*>(piece + k4_ks(p.sm, HD) + (key * G::NG + t) * 4);
+            const unsigned w = *reinterpret_cast<const unsigned*>(piece + k4_k_word<HD>((int)key, t, g));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int kn = (kw >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
-            const int ch = 8 * c8 + e;
-            const unsigned vw = *reinterpret_cast<const unsigned*>(piece + k4_v(p.sm, HD) + k4_v_word<HD>((int)(key >> 5), ch >> 4, vg, ch & 15));
-            const int vn = (vw >> (4 * vj)) & 15;
-            if (p.k) store_from_f32(p.k, ko + e, p.dtype, fmaf(k4_scale(ks), (float)kn, k4_offset(ks)));
-            if (p.v) store_from_f32(p.v, vo + e, p.dtype, fmaf(k4_scale(vs), (float)vn, k4_offset(vs)));
+            for (int e = 0; e < 4; ++e) {
+                const int i = (c4 & 4) + e;
+                x[e] = fmaf(k4_scale(sw), (float)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u), k4_offset(sw));
+            }
+            put(p.k, (long)b * p.k_bs + (long)h * p.k_hs + src * p.k_ss + c4, x);
+        }
+        if (p.v) {
+            const unsigned sw = *reinterpret_cast<const unsigned*>(piece + k4_vs(p.sm, HD) + (key * G::NG + t) * 4);
+            const int vg = (int)(key & 15) >> 2, shift = 4 * ((int)(key & 3) + 4 * (int)((key >> 4) & 1));
+            const char* vw = piece + k4_v(p.sm, HD) + k4_v_word<HD>((int)(key >> 5), c4 >> 4, vg, c4 & 15);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = fmaf(k4_scale(sw), (float)((*reinterpret_cast<const unsigned*>(vw + e * (G::DW * 4)) >> shift) & 15u), k4_offset(sw));
+            put(p.v, (long)b * p.v_bs + (long)h * p.v_hs + src * p.v_ss + c4, x);
         }
     }
 }
@@ -423,26 +436,9 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
     }
 }
 
-// the parts of every row, in order; four columns per thread
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_join_kernel(T* o, const float* part_o, const float* part_ml, long rows, int hd, int nsplit) {
-    const long u = (long)blockIdx.x * 256 + threadIdx.x;
-    const long row = u / (hd / 4);
-    if (row >= rows) return;
-    const int c = (int)(u - row * (hd / 4)) * 4;
-    float mm = -INFINITY, ll = 0.f;
-    for (int s = 0; s < nsplit; ++s) mm = fmaxf(mm, part_ml[2 * (s * rows + row)]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (mm != -INFINITY)
-        for (int s = 0; s < nsplit; ++s) {
-            const float ms = part_ml[2 * (s * rows + row)];
-            const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - mm) * LOG2E);
-            ll += w * part_ml[2 * (s * rows + row) + 1];
-            v += w * *reinterpret_cast<const f32x4*>(part_o + (s * rows + row) * hd + c);
-        }
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[row * hd + c + e] = from_f32<T>(v[e] * inv);
+    join_parts<T>(part_o, part_ml, rows, blockIdx.x, hd, nsplit, o + (long)blockIdx.x * hd, nullptr);
 }
 
 int dec4_splits(int B, int H, int Hkv, int smax, int window, int prefix) {
@@ -452,6 +448,7 @@ int dec4_splits(int B, int H, int Hkv, int smax, int window, int prefix) {
     long ns = (1024 + wgs - 1) / wgs;                        // four workgroups per CU, none with fewer than four blocks for each wave
     const long most = (seen / 32 + 2) / 16;
     if (ns > most) ns = most;
+    if (ns > 1024) ns = 1024;
     return (int)(ns < 1 ? 1 : ns);
 }
 
@@ -465,7 +462,7 @@ template <typename T, int HD> int dec4_launch(const Dec4Args& a, hipStream_t st)
     CAPDEC_LAUNCH_CHECK();
     if (a.nsplit > 1) {
         const long rows = (long)a.B * a.H;
-        hipLaunchKernelGGL((kv4_join_kernel<T>), dim3((unsigned)((rows * (HD / 4) + 255) / 256)), dim3(256), 0, st, (T*)a.o, a.part_o, a.part_ml, rows, HD, a.nsplit);
+        hipLaunchKernelGGL((kv4_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, (T*)a.o, a.part_o, a.part_ml, rows, HD, a.nsplit);
         CAPDEC_LAUNCH_CHECK();
     }
     return CAPDEC_OK;
@@ -530,15 +527,21 @@ extern "C" int capdec_kv4_unpack(const void* cache, const capdec_kv4_rows* r, in
     CAPDEC_CHECK(r->dtype == CAPDEC_BF16 || r->dtype == CAPDEC_F32, "kv4_unpack: bad dtype");
     CAPDEC_CHECK(starts || (start >= 0 && (long)start + r->n <= smax), "kv4_unpack: rows %d..%ld outside a cache of %d", start, (long)start + r->n, smax);
     UnpackArgs a = {(const char*)cache, smax, (smax + 31L) / 32 * 32, B, Hkv, r->n, start, starts, (void*)r->k, (void*)r->v,
-                    r->k_bs, r->k_hs, r->k_ss, r->v_bs, r->v_hs, r->v_ss, r->dtype};
-    const long per = ((long)r->n * hd / 8 + 255) / 256;
+                    r->k_bs, r->k_hs, r->k_ss, r->v_bs, r->v_hs, r->v_ss};
+    const int per16 = r->dtype == CAPDEC_BF16 ? 8 : 4;
+    const long strides[] = {r->k_bs, r->k_hs, r->k_ss, r->v_bs, r->v_hs, r->v_ss};
+    for (long s : strides) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "kv4_unpack: stride %ld (must be a non-negative multiple of %d elements)", s, per16);
+    CAPDEC_CHECK(aligned16(r->k) && aligned16(r->v), "kv4_unpack: rows must be 16-byte aligned");
+    const long per = ((long)r->n * (hd / 4) + 255) / 256;
     const dim3 grid((unsigned)(B * Hkv), (unsigned)(per < 4096 ? per : 4096));
     hipStream_t st = (hipStream_t)stream;
-    switch (hd) {
-        case 32: hipLaunchKernelGGL((kv4_unpack_kernel<32>), grid, dim3(256), 0, st, a); break;
-        case 64: hipLaunchKernelGGL((kv4_unpack_kernel<64>), grid, dim3(256), 0, st, a); break;
-        case 96: hipLaunchKernelGGL((kv4_unpack_kernel<96>), grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL((kv4_unpack_kernel<128>), grid, dim3(256), 0, st, a);
+    auto go = [&](auto kfn) { hipLaunchKernelGGL(kfn, grid, dim3(256), 0, st, a); };
+    if (r->dtype == CAPDEC_BF16) {
+        if (hd == 32) go(kv4_unpack_kernel<bf16_t, 32>); else if (hd == 64) go(kv4_unpack_kernel<bf16_t, 64>);
+        else if (hd == 96) go(kv4_unpack_kernel<bf16_t, 96>); else go(kv4_unpack_kernel<bf16_t, 128>);
+    } else {
+        if (hd == 32) go(kv4_unpack_kernel<float, 32>); else if (hd == 64) go(kv4_unpack_kernel<float, 64>);
+        else if (hd == 96) go(kv4_unpack_kernel<float, 96>); else go(kv4_unpack_kernel<float, 128>);
     }
     CAPDEC_LAUNCH_CHECK();
     return CAPDEC_OK;

@@ -214,31 +214,14 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     }
 }
 
-// o and lse of every row from its nsplit parts; four columns per thread, the parts in a fixed order
+// o and lse of every row from its nsplit parts: one workgroup per row
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void win_join_kernel(WinArgs p) {
-    const long rows_all = (long)p.B * p.Hkv * p.rows;
-    const long u = (long)blockIdx.x * 256 + threadIdx.x;
-    const long row = u / (HD / 4);
-    if (row >= rows_all) return;
-    const int c = (int)(u - row * (HD / 4)) * 4;
-    float mm = -INFINITY, ll = 0.f;
-    for (int s = 0; s < p.nsplit; ++s) mm = fmaxf(mm, p.part_ml[2 * (s * rows_all + row)]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (mm != -INFINITY)
-        for (int s = 0; s < p.nsplit; ++s) {
-            const float ms = p.part_ml[2 * (s * rows_all + row)];
-            const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - mm) * WIN_LOG2E);
-            ll += w * p.part_ml[2 * (s * rows_all + row) + 1];
-            v += w * *reinterpret_cast<const f32x4*>(p.part_o + (s * rows_all + row) * HD + c);
-        }
+    const long row = blockIdx.x;
     const int bh = (int)(row / p.rows), r = (int)(row - (long)bh * p.rows);
     const int b = bh / p.Hkv, i = win_row_query(p, r), h = (bh - b * p.Hkv) * p.G + r - i * p.G;
-    T* at = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_ss + c;
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) at[e] = from_f32<T>(v[e] * inv);
-    if (c == 0 && p.lse) p.lse[((long)b * p.H + h) * p.nq + i] = ll != 0.f ? mm + logf(ll) : -INFINITY;
+    join_parts<T>(p.part_o, p.part_ml, (long)p.B * p.Hkv * p.rows, row, HD, p.nsplit,
+                  reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_ss, p.lse ? p.lse + ((long)b * p.H + h) * p.nq + i : nullptr);
 }
 
 template <typename T, int HD, int QW, int KW, int NSUB, bool DROP>
@@ -254,8 +237,7 @@ int fwd_go(WinArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(kfn, dim3((unsigned)grid), dim3(64 * QW * KW), lds, st, a);
     CAPDEC_LAUNCH_CHECK();
     if (a.nsplit > 1) {
-        const long threads = (long)a.B * a.Hkv * a.rows * (HD / 4);
-        hipLaunchKernelGGL((win_join_kernel<T, HD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((win_join_kernel<T, HD>), dim3((unsigned)((long)a.B * a.Hkv * a.rows)), dim3(256), 0, st, a);
         CAPDEC_LAUNCH_CHECK();
     }
     return CAPDEC_OK;
@@ -338,6 +320,7 @@ WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window
     if (wgs < 512) {                     // two workgroups per CU, each with at least four key tiles of its own
         ns = (512 + wgs - 1) / wgs;
         if (ns > nt / 4) ns = nt / 4;
+        if (ns > 1024) ns = 1024;
         if (ns < 1) ns = 1;
     }
     pl.nsplit = (int)ns;

@@ -297,15 +297,14 @@ int capdec_attn_window_decode(const void* q, const void* kv_cache, void* o, int 
 long capdec_kv4_head_bytes(int smax, int hd);
 
 /* n rows per sequence, k/v [B,Hkv,n,hd] of dtype addressed as base + b*bs + h*hs + s*ss + j (elements).  For
- * capdec_kv4_unpack they are written, and one of k / v may be NULL. */
+ * capdec_kv4_unpack they are written, and one of k / v may be NULL.  Rows 16-byte aligned, strides multiples of 16 bytes. */
 typedef struct {
     const void* k; const void* v;
     long k_bs, k_hs, k_ss;  long v_bs, v_hs, v_ss;
     int dtype, n;
 } capdec_kv4_rows;
 
-/* Quantises n new rows of every sequence into rows start.. of the cache (rows 16-byte aligned, strides multiples of 16
- * bytes).  starts [B] int32 on the device (NULL: `start` for all): where each sequence's rows go; rows that would fall outside
+/* Quantises n new rows of every sequence into rows start.. of the cache.  starts [B] int32 on the device (NULL: `start` for all): where each sequence's rows go; rows that would fall outside
  * 0..smax-1 are dropped.  counts [B] int32 on the device (NULL: n for all): how many of the n rows each sequence has, taken
  * into 0..n.  Other rows of the cache keep what they hold.  Two calls that may overlap in time must not write the same
  * 32-row block of a sequence. */
