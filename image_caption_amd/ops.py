@@ -287,40 +287,53 @@ def attn_decode(q, kv_cache, o, B, H, hd, smax, length):
           "capdec_attn_decode")
 
 
-def _need(cond: bool, what: str):
+def _need(cond: bool, what: str, *args):
+    """ValueError(what.format(*args)) unless cond; formatted only then (these checks run once per token)."""
     if not cond:
-        raise ValueError(what)
+        raise ValueError(what.format(*args))
 
 
-def _on_current_device(*tensors):
+def _on_current_device(*tensors) -> int:
     """The launch goes to the current device's current stream: a tensor of another device must not reach it."""
-    require_cuda(*tensors)
-    cur = torch.cuda.current_device()
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
     for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise RuntimeError(f"a tensor on {t.device} was passed while cuda:{cur} is the current device")
+        if t is not None and (t.get_device() != dev or dev < 0):
+            require_cuda(t)
+            raise RuntimeError(f"a tensor on {t.device} was passed while cuda:{dev} is the current device")
+    return dev
 
 
-def _bhsd(t, name, shape, dtype, *, written=False):
+def _raw_stream(dev: int) -> int:
+    """The current stream of a device, without building a Stream object (7 us of a 14 us call for one token)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _bhsd(t, name, shape, dtype, written=False):
     """(batch, head, row) strides of a [B, heads, rows, hd] view with unit inner stride; an axis of one element counts as 0."""
-    _need(t.dim() == 4 and tuple(t.shape) == tuple(shape) and t.dtype == dtype, f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
-    _need(t.stride(3) == 1, f"{name} needs unit stride along its last axis")
-    if written:
-        _need(all(t.stride(i) > 0 or t.shape[i] == 1 for i in range(3)), f"{name} is written: its rows must not overlap")
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3))
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
+    b, h, s, one = t.stride()
+    B, H, S, _ = shape
+    if one != 1 and shape[3] > 1:
+        raise ValueError(f"{name} needs unit stride along its last axis")
+    b, h, s = (b if B > 1 else 0), (h if H > 1 else 0), (s if S > 1 else 0)
+    if written and not ((b or B <= 1) and (h or H <= 1) and (s or S <= 1)):
+        raise ValueError(f"{name} is written: its rows must not overlap")
+    return b, h, s
 
 
 def _lens_ptr(lens, B):
-    if lens is not None:
-        _need(lens.dtype == torch.int32 and tuple(lens.shape) == (B,) and lens.is_contiguous(), f"lens must be a contiguous int32 [{B}] tensor")
-    return ptr(lens)
+    if lens is None:
+        return None
+    _need(lens.dtype == torch.int32 and lens.dim() == 1 and lens.shape[0] == B and lens.is_contiguous(), "lens must be a contiguous int32 [{}] tensor", B)
+    return lens.data_ptr()
 
 
 def _ws(workspace):
     if workspace is None:
         return None, 0
     _need(workspace.is_contiguous(), "workspace must be contiguous")
-    return ptr(workspace), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> int:
@@ -328,26 +341,18 @@ def attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> 
     return _lib.load().capdec_attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
 
 
-def _fill_window(desc, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, *, o_written):
+def _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written):
     _on_current_device(q, k, v, o, lens, lse, workspace)
     _need(q.dim() == 4 and k.dim() == 4, "q must be [B, H, nq, hd] and k [B, Hkv, S, hd]")
-    B, H, nq, hd = q.shape
+    shape, dtype = q.shape, q.dtype
+    B, H, nq, hd = shape
     Hkv, S = k.shape[1], k.shape[2]
-    desc.q, desc.k, desc.v, desc.o = ptr(q), ptr(k), ptr(v), ptr(o)
-    desc.q_bs, desc.q_hs, desc.q_ss = _bhsd(q, "q", (B, H, nq, hd), q.dtype)
-    desc.k_bs, desc.k_hs, desc.k_ss = _bhsd(k, "k", (B, Hkv, S, hd), q.dtype)
-    desc.v_bs, desc.v_hs, desc.v_ss = _bhsd(v, "v", (B, Hkv, S, hd), q.dtype)
-    desc.o_bs, desc.o_hs, desc.o_ss = _bhsd(o, "o", (B, H, nq, hd), q.dtype, written=o_written)
+    kv = (B, Hkv, S, hd)
     if lse is not None:
-        _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, nq) and lse.is_contiguous(), f"lse must be a contiguous float32 {[B, H, nq]} tensor")
-    desc.dtype = dtype_code(q)
-    desc.B, desc.H, desc.Hkv, desc.S, desc.hd = B, H, Hkv, S, hd
-    desc.q_start, desc.nq = q_start, nq
-    desc.window, desc.prefix_len, desc.prefix_open = window, prefix_len, int(prefix_open)
-    desc.lens = _lens_ptr(lens, B)
-    desc.drop = drop
-    desc.lse = ptr(lse)
-    desc.workspace, desc.workspace_bytes = _ws(workspace)
+        _need(lse.dtype == torch.float32 and lse.shape == (B, H, nq) and lse.is_contiguous(), "lse must be a contiguous float32 [{}, {}, {}] tensor", B, H, nq)
+    return AttnWindowDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                          *_bhsd(q, "q", shape, dtype), *_bhsd(k, "k", kv, dtype), *_bhsd(v, "v", kv, dtype), *_bhsd(o, "o", shape, dtype, o_written),
+                          dtype_code(q), B, H, Hkv, S, hd, q_start, nq, window, prefix_len, int(prefix_open), _lens_ptr(lens, B), drop, ptr(lse), *_ws(workspace))
 
 
 def attn_window_fwd(q, k, v, o, *, window, prefix_len=0, prefix_open=False, q_start=0, lens=None, drop: Dropout = NO_DROPOUT, lse=None,
@@ -356,11 +361,10 @@ def attn_window_fwd(q, k, v, o, *, window, prefix_len=0, prefix_open=False, q_st
     position q_start + r), k, v [B, Hkv, S, hd], any strides along the first three axes.  window counts the query's own key
     (0: no limit); prefix_open lets queries before the prefix's end see all of it.  lens [B] int32: rows of each sequence;
     lse [B, H, nq] f32 (optional) for the backward.  A query at or past its sequence's end gives 0 and lse -inf."""
-    desc = AttnWindowDesc()
-    _fill_window(desc, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written=True)
+    desc = _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, True)
     if q.numel() == 0:
         return o
-    check(_lib.load().capdec_attn_window_fwd(C.byref(desc), _st()), "capdec_attn_window_fwd")
+    check(_lib.load().capdec_attn_window_fwd(C.byref(desc), _raw_stream(q.get_device())), "capdec_attn_window_fwd")
     return o
 
 
@@ -372,28 +376,22 @@ def attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, delta, *, window, prefix_
                     drop: Dropout = NO_DROPOUT, dq_scale=1.0, workspace=None):
     """Gradients of attn_window_fwd (o and lse as it wrote them): dq [B, H, nq, hd], dk / dv [B, Hkv, S, hd], every row
     written; delta [B, H, nq] f32 scratch.  workspace: attn_window_bwd_workspace bytes (allocated here if None)."""
-    desc = AttnWindowBwdDesc()
+    _need(lse is not None, "the backward needs the forward's lse")
     if workspace is None and q.dim() == 4 and k.dim() == 4 and q.is_cuda:
         B, H, nq, hd = q.shape
         workspace = torch.empty(attn_window_bwd_workspace(B, H, k.shape[1], k.shape[2], nq, hd, window=window, prefix_len=prefix_len),
                                 dtype=torch.uint8, device=q.device)
-    _need(lse is not None, "the backward needs the forward's lse")
-    _fill_window(desc.fwd, q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written=False)
+    fwd = _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, False)
     _on_current_device(dout, dq, dk, dv, delta)
-    B, H, nq, hd = q.shape
-    Hkv, S = k.shape[1], k.shape[2]
-    desc.dout, (desc.do_bs, desc.do_hs, desc.do_ss) = ptr(dout), _bhsd(dout, "dout", (B, H, nq, hd), q.dtype)
-    desc.dq, (desc.dq_bs, desc.dq_hs, desc.dq_ss) = ptr(dq), _bhsd(dq, "dq", (B, H, nq, hd), q.dtype, written=True)
-    desc.dk, (desc.dk_bs, desc.dk_hs, desc.dk_ss) = ptr(dk), _bhsd(dk, "dk", (B, Hkv, S, hd), q.dtype, written=True)
-    desc.dv, (desc.dv_bs, desc.dv_hs, desc.dv_ss) = ptr(dv), _bhsd(dv, "dv", (B, Hkv, S, hd), q.dtype, written=True)
-    _need(delta.dtype == torch.float32 and delta.numel() == B * H * nq and delta.is_contiguous(), "delta must be contiguous float32 scratch of B * H * nq")
-    desc.dq_scale = dq_scale
-    desc.delta = ptr(delta)
+    shape, kv, dtype = q.shape, k.shape, q.dtype
+    _need(delta.dtype == torch.float32 and delta.numel() == shape[0] * shape[1] * shape[2] and delta.is_contiguous(), "delta must be contiguous float32 scratch of B * H * nq")
+    desc = AttnWindowBwdDesc(fwd, ptr(dout), *_bhsd(dout, "dout", shape, dtype), ptr(dq), *_bhsd(dq, "dq", shape, dtype, True),
+                             ptr(dk), *_bhsd(dk, "dk", kv, dtype, True), ptr(dv), *_bhsd(dv, "dv", kv, dtype, True), dq_scale, ptr(delta))
     if q.numel() == 0:                      # no queries: nothing reaches a key
         dk.zero_()
         dv.zero_()
         return
-    check(_lib.load().capdec_attn_window_bwd(C.byref(desc), _st()), "capdec_attn_window_bwd")
+    check(_lib.load().capdec_attn_window_bwd(C.byref(desc), _raw_stream(q.get_device())), "capdec_attn_window_bwd")
 
 
 def attn_window_decode_workspace(B, H, Hkv, hd, smax, *, window, prefix_len=0) -> int:
@@ -403,7 +401,7 @@ def attn_window_decode_workspace(B, H, Hkv, hd, smax, *, window, prefix_len=0) -
 def attn_window_decode(q, kv_cache, o, *, window, prefix_len=0, length=None, lens=None, workspace=None):
     """One query per sequence, its last position, over kv_cache [B, Hkv, 2, smax, hd]: q, o [B, H, hd] (or [B, H * hd]).
     length: rows of every sequence (default smax); lens [B] int32 (optional): of each, at most length."""
-    _on_current_device(q, kv_cache, o, lens, workspace)
+    dev = _on_current_device(q, kv_cache, o, lens, workspace)
     _need(kv_cache.dim() == 5 and kv_cache.shape[2] == 2 and kv_cache.is_contiguous(), "kv_cache must be a contiguous [B, Hkv, 2, smax, hd] tensor")
     B, Hkv, _, smax, hd = kv_cache.shape
     H = _decode_heads(q, o, B, hd)
@@ -412,59 +410,54 @@ def attn_window_decode(q, kv_cache, o, *, window, prefix_len=0, length=None, len
         return o
     wp, wb = _ws(workspace)
     check(_lib.load().capdec_attn_window_decode(ptr(q), ptr(kv_cache), ptr(o), dtype_code(q), B, H, Hkv, hd, smax, smax if length is None else length,
-                                                _lens_ptr(lens, B), window, prefix_len, wp, wb, _st()), "capdec_attn_window_decode")
+                                                _lens_ptr(lens, B), window, prefix_len, wp, wb, _raw_stream(dev)), "capdec_attn_window_decode")
     return o
 
 
 def _decode_heads(q, o, B, hd):
     _need(q.is_contiguous() and o.is_contiguous() and q.shape == o.shape and q.dtype == o.dtype, "q and o must be contiguous, of one shape and dtype")
-    _need(q.dim() in (2, 3) and q.shape[0] == B and q[0:1].numel() % hd == 0 and (q.dim() == 2 or q.shape[2] == hd), f"q must be [{B}, H, {hd}] or [{B}, H * {hd}]")
+    _need(q.dim() in (2, 3) and q.shape[0] == B and q[0:1].numel() % hd == 0 and (q.dim() == 2 or q.shape[2] == hd), "q must be [{0}, H, {1}] or [{0}, H * {1}]", B, hd)
     return q.shape[1] if q.dim() == 3 else q.shape[1] // hd
 
 
 def kv4_cache(B, Hkv, smax, hd, device) -> torch.Tensor:
     """An empty cache of smax rows per sequence in 4 bits per value: [B, Hkv, bytes] uint8 (the layout is the library's own)."""
     size = _lib.load().capdec_kv4_head_bytes(smax, hd)
-    _need(size > 0, f"no 4-bit cache of {smax} rows of {hd} channels (32, 64, 96 or 128)")
+    _need(size > 0, "no 4-bit cache of {} rows of {} channels (32, 64, 96 or 128)", smax, hd)
     return torch.zeros(B, Hkv, size, dtype=torch.uint8, device=device)
 
 
 def _kv4_geometry(cache, smax, hd):
     _need(cache.dim() == 3 and cache.dtype == torch.uint8 and cache.is_contiguous() and
-          cache.shape[2] == _lib.load().capdec_kv4_head_bytes(smax, hd) > 0, f"cache must come from kv4_cache(B, Hkv, {smax}, {hd}, device)")
+          cache.shape[2] == _lib.load().capdec_kv4_head_bytes(smax, hd) > 0, "cache must come from kv4_cache(B, Hkv, {}, {}, device)", smax, hd)
     return cache.shape[0], cache.shape[1]
 
 
-def _kv4_rows(k, v, B, Hkv, *, written=False):
+def _kv4_rows(k, v, B, Hkv, written=False):
     t = k if k is not None else v
     _need(t is not None and t.dim() == 4, "k and v must be [B, Hkv, n, hd]")
-    shape = (B, Hkv, t.shape[2], t.shape[3])
-    r = _lib.Kv4Rows()
-    if k is not None:
-        r.k, (r.k_bs, r.k_hs, r.k_ss) = ptr(k), _bhsd(k, "k", shape, t.dtype, written=written)
-    if v is not None:
-        r.v, (r.v_bs, r.v_hs, r.v_ss) = ptr(v), _bhsd(v, "v", shape, t.dtype, written=written)
-    r.dtype, r.n = dtype_code(t), t.shape[2]
-    return r
+    shape, dtype = (B, Hkv, t.shape[2], t.shape[3]), t.dtype
+    return _lib.Kv4Rows(ptr(k), ptr(v), *(_bhsd(k, "k", shape, dtype, written) if k is not None else (0, 0, 0)),
+                        *(_bhsd(v, "v", shape, dtype, written) if v is not None else (0, 0, 0)), dtype_code(t), t.shape[2])
 
 
 def kv4_append(k, v, cache, *, smax, start=0, starts=None, counts=None):
     """Quantises the rows k, v [B, Hkv, n, hd] into rows start.. (or starts[b]..) of a kv4_cache; counts[b] (optional): how many
     of the n rows sequence b has.  With starts, rows that would fall outside the cache are dropped."""
-    _on_current_device(k, v, cache, starts, counts)
+    dev = _on_current_device(k, v, cache, starts, counts)
     _need(k.dim() == 4, "k and v must be [B, Hkv, n, hd]")
     B, Hkv = _kv4_geometry(cache, smax, k.shape[3])
     rows = _kv4_rows(k, v, B, Hkv)
     sp, cp = _lens_ptr(starts, B), _lens_ptr(counts, B)
     if k.numel() == 0:
         return cache
-    check(_lib.load().capdec_kv4_append(C.byref(rows), ptr(cache), B, Hkv, smax, k.shape[3], start, sp, cp, _st()), "capdec_kv4_append")
+    check(_lib.load().capdec_kv4_append(C.byref(rows), ptr(cache), B, Hkv, smax, k.shape[3], start, sp, cp, _raw_stream(dev)), "capdec_kv4_append")
     return cache
 
 
 def kv4_unpack(cache, k_out, v_out, *, smax, start=0, starts=None):
     """The values that rows start.. (or starts[b]..) of a kv4_cache stand for, into k_out / v_out [B, Hkv, n, hd] (one may be None)."""
-    _on_current_device(cache, k_out, v_out, starts)
+    dev = _on_current_device(cache, k_out, v_out, starts)
     t = k_out if k_out is not None else v_out
     _need(t is not None and t.dim() == 4, "k_out and v_out must be [B, Hkv, n, hd]")
     B, Hkv = _kv4_geometry(cache, smax, t.shape[3])
@@ -472,7 +465,7 @@ def kv4_unpack(cache, k_out, v_out, *, smax, start=0, starts=None):
     sp = _lens_ptr(starts, B)
     if t.numel() == 0:
         return
-    check(_lib.load().capdec_kv4_unpack(ptr(cache), C.byref(rows), B, Hkv, smax, t.shape[3], start, sp, _st()), "capdec_kv4_unpack")
+    check(_lib.load().capdec_kv4_unpack(ptr(cache), C.byref(rows), B, Hkv, smax, t.shape[3], start, sp, _raw_stream(dev)), "capdec_kv4_unpack")
 
 
 def attn_decode_kv4_workspace(B, H, Hkv, hd, smax, *, window=0, prefix_len=0) -> int:
@@ -481,7 +474,7 @@ def attn_decode_kv4_workspace(B, H, Hkv, hd, smax, *, window=0, prefix_len=0) ->
 
 def attn_decode_kv4(q, cache, o, *, smax, window=0, prefix_len=0, length=None, lens=None, workspace=None):
     """attn_window_decode over a kv4_cache: q, o [B, H, hd]; every key is visible unless a window is given."""
-    _on_current_device(q, cache, o, lens, workspace)
+    dev = _on_current_device(q, cache, o, lens, workspace)
     _need(q.dim() == 3, "q must be [B, H, hd]")
     hd = q.shape[2]
     B, Hkv = _kv4_geometry(cache, smax, hd)
@@ -490,7 +483,7 @@ def attn_decode_kv4(q, cache, o, *, smax, window=0, prefix_len=0, length=None, l
         return o
     wp, wb = _ws(workspace)
     check(_lib.load().capdec_attn_decode_kv4(ptr(q), ptr(cache), ptr(o), dtype_code(q), B, H, Hkv, hd, smax, smax if length is None else length,
-                                             _lens_ptr(lens, B), window, prefix_len, wp, wb, _st()), "capdec_attn_decode_kv4")
+                                             _lens_ptr(lens, B), window, prefix_len, wp, wb, _raw_stream(dev)), "capdec_attn_decode_kv4")
     return o
 
 
