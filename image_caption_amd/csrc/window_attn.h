@@ -67,10 +67,46 @@ __device__ __forceinline__ int win_xcd_id(int w, int n) {
     return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (w >> 3);
 }
 
+// Rows in LDS: PB bytes each, no padding, their 16-byte chunks permuted by the row (win_chunk) so that neither kind of read
+// meets itself in a bank: mma_rows reads one chunk of 32 rows (eight rows to a 128-byte phase), mma_cols two neighbouring
+// chunks of four rows.  With a pad of 16 bytes the second kind alone cost 42 % of the LDS cycles.
+//   rows of whole 128 bytes:  chunk ^ f,  f = (row & 3) << 1 | (row >> 2 & 1): all of 0..7 over eight rows, and four different
+//                             pairs over four;
+//   rows of 64 or 192 bytes (bf16, 32 or 96 channels): consecutive rows already lie half a phase apart; the low two bits are
+//                             XORed with the reversed bits of row >> 1.
 template <typename T, int HD> struct WinGeo {
-    static constexpr int PB = HD * (int)sizeof(T) + 16;          // LDS bytes per row: an odd number of 16-byte units
-    static constexpr int CPR = HD * (int)sizeof(T) / 16;         // 16-byte chunks per row
+    static constexpr int PB = HD * (int)sizeof(T);
+    static constexpr int CPR = PB / 16;                          // 16-byte chunks per row
     static constexpr int DT = HD / 32;
+    static constexpr bool WHOLE = PB % 128 == 0;
+    static __device__ __forceinline__ int mix(int row) {
+        return WHOLE ? (row & 3) << 1 | (row >> 2 & 1) : (row >> 1 & 1) << 1 | (row >> 2 & 1);
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * PB + ((chunk ^ mix(row)) << 4); }
+};
+// byte offsets of what a lane reads for mma_rows (chunk 2 s + (lane >> 5) of row lane & 31): the XOR leaves P addresses, the
+// other steps lie a constant further on
+template <typename T, int HD> struct RowAt {
+    using G = WinGeo<T, HD>;
+    static constexpr int P = G::WHOLE ? 4 : 2;
+    int at[P];
+    __device__ __forceinline__ RowAt(int lane) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) at[i] = G::at(lane & 31, 2 * i + (lane >> 5));
+    }
+    __device__ __forceinline__ int operator()(int s) const { return at[s % P] + (s / P) * (32 * P); }
+};
+// the same for the transposing read of mma_cols: four rows 4 (lane >> 5) .. of columns 16 (lane >> 4 & 1) .. + 15 of tile dt
+template <int HD> struct ColAt {
+    using G = WinGeo<bf16_t, HD>;
+    static constexpr int P = G::WHOLE ? 2 : 1;
+    int at[P];
+    __device__ __forceinline__ ColAt(int lane) {
+        const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
+#pragma unroll
+        for (int t = 0; t < P; ++t) at[t] = G::at(row, 4 * t + 2 * (g & 1) + ((i & 3) >> 1)) + 8 * (i & 1);
+    }
+    __device__ __forceinline__ int operator()(int dt) const { return at[dt % P] + (dt / P) * (64 * P); }
 };
 
 // one row per lane (row = lane & 31; the two halves of the wave hold alternate pieces of it), as mma_rows wants it
@@ -125,45 +161,52 @@ template <int HD> struct RowFrag<float, HD> {
     }
 };
 
-template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<bf16_t, HD>& b, int lane) {
-    const char* at = lds + (lane & 31) * WinGeo<bf16_t, HD>::PB + (lane >> 5) * 16;
+// where a lane reads in a tile: computed once per kernel
+template <typename T, int HD> struct LaneAt;
+template <int HD> struct LaneAt<bf16_t, HD> {
+    RowAt<bf16_t, HD> row;
+    ColAt<HD> col;
+    __device__ __forceinline__ LaneAt(int lane) : row(lane), col(lane) {}
+};
+template <int HD> struct LaneAt<float, HD> {
+    RowAt<float, HD> row;
+    int lane;
+    __device__ __forceinline__ LaneAt(int lane_) : row(lane_), lane(lane_) {}
+};
+
+template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<bf16_t, HD>& b, const LaneAt<bf16_t, HD>& at) {
 #pragma unroll
     for (int s = 0; s < HD / 16; ++s)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(at + 32 * s), b.f[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(lds + at.row(s)), b.f[s], acc, 0, 0, 0);
 }
-template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<float, HD>& b, int lane) {
-    const char* at = lds + (lane & 31) * WinGeo<float, HD>::PB + (lane >> 5) * 16;
+template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<float, HD>& b, const LaneAt<float, HD>& at) {
 #pragma unroll
     for (int s = 0; s < HD / 8; ++s) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(at + 32 * s);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at.row(s));
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b.f[s][e], acc, 0, 0, 0);
     }
 }
 
 // the same with the second operand's rows in LDS as well
-template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, bf16_t, int lane) {
-    const int at = (lane & 31) * WinGeo<bf16_t, HD>::PB + (lane >> 5) * 16;
+template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, const LaneAt<bf16_t, HD>& at) {
 #pragma unroll
     for (int s = 0; s < HD / 16; ++s)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(lds + at + 32 * s), *reinterpret_cast<const bf16x8*>(rows + at + 32 * s),
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(lds + at.row(s)), *reinterpret_cast<const bf16x8*>(rows + at.row(s)),
                                                       acc, 0, 0, 0);
 }
-template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, float, int lane) {
-    const int at = (lane & 31) * WinGeo<float, HD>::PB + (lane >> 5) * 16;
+template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, const LaneAt<float, HD>& at) {
 #pragma unroll
     for (int s = 0; s < HD / 8; ++s) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at + 32 * s), b = *reinterpret_cast<const f32x4*>(rows + at + 32 * s);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at.row(s)), b = *reinterpret_cast<const f32x4*>(rows + at.row(s));
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
     }
 }
 
 // p is rounded to bf16 (half a step, 2^-8 of each term) to be an operand: the products' own inputs have no more bits
-template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, bf16_t, int lane) {
+template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<bf16_t, HD>& at) {
     constexpr int PB = WinGeo<bf16_t, HD>::PB;
-    const int g = lane >> 4, i = lane & 15;
-    const char* at = lds + (4 * (g >> 1) + (i >> 2)) * PB + (16 * (g & 1) + 4 * (i & 3)) * 2;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         bf16x8 pb;
@@ -171,21 +214,24 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
         for (int e = 0; e < 8; ++e) pb[e] = (bf16_t)p[8 * c + e];
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
-            const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at + (16 * c) * PB + 64 * dt));
-            const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at + (16 * c + 8) * PB + 64 * dt));
+            const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, lds + at.col(dt) + (16 * c) * PB));
+            const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, lds + at.col(dt) + (16 * c + 8) * PB));
             const bf16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
             acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb, acc[dt], 0, 0, 0);
         }
     }
 }
-template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, float, int lane) {
-    constexpr int PB = WinGeo<float, HD>::PB;
-    const char* at = lds + 4 * (lane >> 5) * PB + (lane & 31) * 4;
+template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<float, HD>& at) {
+    using G = WinGeo<float, HD>;
+    const int h = at.lane >> 5, d = at.lane & 31;
 #pragma unroll
     for (int e = 0; e < 16; ++e)
 #pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt)
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(at + (8 * (e >> 2) + (e & 3)) * PB + 128 * dt), p[e], acc[dt], 0, 0, 0);
+        for (int dt = 0; dt < HD / 32; ++dt) {
+            const int row = 8 * (e >> 2) + (e & 3);               // + 4 h: of the row, mix() takes bits 0..2 only
+            const int off = row * G::PB + 4 * h * G::PB + (((8 * dt + (d >> 2)) ^ ((e & 3) << 1 | h)) << 4) + 4 * (d & 3);
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(lds + off), p[e], acc[dt], 0, 0, 0);
+        }
 }
 
 // NROWS rows of two strided matrices on their way to LDS; rows past the end arrive as zeros and are not read
@@ -208,8 +254,8 @@ template <typename T, int HD, int NROWS, int NT> struct TilePair {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
-            *reinterpret_cast<u32x4*>(lds0 + row * WinGeo<T, HD>::PB + ch * 16) = a[j];
-            *reinterpret_cast<u32x4*>(lds1 + row * WinGeo<T, HD>::PB + ch * 16) = b[j];
+            *reinterpret_cast<u32x4*>(lds0 + WinGeo<T, HD>::at(row, ch)) = a[j];
+            *reinterpret_cast<u32x4*>(lds1 + WinGeo<T, HD>::at(row, ch)) = b[j];
         }
     }
 };
@@ -261,6 +307,8 @@ template <int HD> __device__ __forceinline__ void store_rows(const f32x16 (&acc)
 }
 
 // ------------------------------------------------------------------ host side
+// four waves on the keys of 32 rows instead of on 32 rows each: for few rows, and where tiles of 128 rows would leave CUs idle
+inline bool win_few_rows(long bh, long rows) { return rows <= 64 || bh * ((rows + 127) / 128) < 256; }
 int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what);
 struct WinFwdPlan { int kw; int tiles; int nsplit; long part_floats; };   // kw: four waves share the keys of 32 rows (else 4 x 32 rows)
 WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix);

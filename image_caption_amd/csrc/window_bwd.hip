@@ -28,6 +28,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     constexpr bool PRE = KW == 1 || HD < 128;          // the next tile's loads go out before this one's products, where the registers hold them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const LaneAt<T, HD> at(lane);
     const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
     const int id = win_xcd_id(blockIdx.x, gridDim.x);
     const int tile = id % p.tiles, bh = id / p.tiles;
@@ -82,15 +83,15 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     auto compute = [&](int idx, const char* lk0, const char* lv0) {
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
-            const int at = kw * 32 * NSUB + 32 * u, key0 = tl.at(idx) * BK + at;
+            const int off = kw * 32 * NSUB + 32 * u, key0 = tl.at(idx) * BK + off;
             if (key0 >= any_end || (key0 >= any_a && key0 + 32 <= s0.lo)) continue;
-            const char* lk = lk0 + at * G::PB;
-            const char* lv = lv0 + at * G::PB;
+            const char* lk = lk0 + off * G::PB;
+            const char* lv = lv0 + off * G::PB;
             f32x16 s, dp;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-            mma_rows<HD>(s, lk, qf, lane);
-            mma_rows<HD>(dp, lv, df, lane);
+            mma_rows<HD>(s, lk, qf, at);
+            mma_rows<HD>(dp, lv, df, at);
             const bool whole = all_live && (key0 + 32 <= s0.a || (key0 >= s1.lo && key0 + 32 <= s0.hi));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
-            mma_cols<HD>(acc, lk, s, T{}, lane);
+            mma_cols<HD>(acc, lk, s, at);
         }
     };
     if (tl.nt > 0) {
@@ -193,6 +194,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
     constexpr int BUF = 2 * MAT + 3 * RB * 4;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const LaneAt<T, HD> at(lane);
     const int per_bh = p.kp * p.ncp + (p.ktiles - p.kp) * p.ncn;
     const int id = win_xcd_id(blockIdx.x, gridDim.x);
     const int bh = id / per_bh, in = id - bh * per_bh;
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
 #pragma unroll
         for (int j = 0; j < KT * CPR / 256; ++j) {
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
-            *reinterpret_cast<u32x4*>(lk + row * G::PB + ch * 16) = z[j];
+            *reinterpret_cast<u32x4*>(lk + G::at(row, ch)) = z[j];
         }
     }
     vf.landed();
@@ -266,8 +268,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
             if (RB * CPR % 256 == 0 || row < RB) {
                 const u32x4 z = {0, 0, 0, 0};
-                *reinterpret_cast<u32x4*>(buf + row * G::PB + ch * 16) = row < live ? fq[j] : z;
-                *reinterpret_cast<u32x4*>(buf + MAT + row * G::PB + ch * 16) = row < live ? fd[j] : z;
+                *reinterpret_cast<u32x4*>(buf + G::at(row, ch)) = row < live ? fq[j] : z;
+                *reinterpret_cast<u32x4*>(buf + MAT + G::at(row, ch)) = row < live ? fd[j] : z;
             }
         }
         if (tid < RB) {
@@ -287,8 +289,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
         f32x16 s, dp;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-        mma_rows_lds<HD>(s, buf, lkw, T{}, lane);
-        mma_rows<HD>(dp, buf + MAT, vf, lane);
+        mma_rows_lds<HD>(s, buf, lkw, at);
+        mma_rows<HD>(dp, buf + MAT, vf, at);
         const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
         const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
 #pragma unroll
@@ -319,8 +321,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
             for (int e = 0; e < 16; ++e) {
                 const int r = min(ra + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), p.rows - 1);
                 const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
-                const uint32_t at = (uint32_t)((((long)b * p.H + h) * p.S + p.q_start + i) * p.S4) + (uint32_t)key;
-                const float f = dropout_keep(p.drop_k0, p.drop_k1, at, p.drop_thr) ? p.drop_scale : 0.f;
+                const uint32_t idx = (uint32_t)((((long)b * p.H + h) * p.S + p.q_start + i) * p.S4) + (uint32_t)key;
+                const float f = dropout_keep(p.drop_k0, p.drop_k1, idx, p.drop_thr) ? p.drop_scale : 0.f;
                 pd[e] *= f;
                 dp[e] *= f;
             }
@@ -331,8 +333,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * jj + e] *= dp[4 * jj + e] - delta[e];
         }
-        mma_cols<HD>(dv, buf + MAT, pd, T{}, lane);
-        mma_cols<HD>(dk, buf, s, T{}, lane);
+        mma_cols<HD>(dv, buf + MAT, pd, at);
+        mma_cols<HD>(dk, buf, s, at);
     };
     if (b_begin < b_end) {
         fetch(b_begin);
@@ -394,10 +396,12 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
     const long all = (rows + RB - 1) / RB;                                 // row blocks a prefix tile sees
     long band = ((w + KT) * G + RB - 1) / RB;                              // and another one
     if (band > all) band = all;
-    // enough workgroups for two per CU, none with fewer than 16 steps for it
-    auto chunks = [](long wgs, long steps) {
+    // enough workgroups for two per CU; a chunk's partial sums cost about what two steps do, so none has fewer than 16 steps
+    // -- unless the tiles do not even give every other CU a workgroup, where latency counts: two
+    const long least = bh * pl.ktiles < 128 ? 2 : 16;
+    auto chunks = [least](long wgs, long steps) {
         long c = wgs > 0 ? (512 + wgs - 1) / wgs : 1;
-        if (c > steps / 16) c = steps / 16;
+        if (c > steps / least) c = steps / least;
         return (int)(c < 1 ? 1 : c);
     };
     pl.ncn = chunks(bh * pl.ktiles, band);
@@ -412,8 +416,8 @@ template <typename T, int HD, bool DROP>
 int bwd_go(WinArgs& a, hipStream_t st) {
     using G = WinGeo<T, HD>;
     const long bh = (long)a.B * a.Hkv;
-    {   // dQ: four waves on the keys of 32 rows when there are few rows
-        const bool kw = a.rows <= 64;
+    {
+        const bool kw = win_few_rows(bh, a.rows);
         constexpr int NS = sizeof(T) == 2 ? 2 : 1;
         a.tiles = (a.rows + (kw ? 31 : 127)) / (kw ? 32 : 128);
         CAPDEC_CHECK(bh * a.tiles < (1L << 31), "attn_window_bwd: grid too large");

@@ -26,6 +26,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     constexpr bool PRE = KW == 1 || HD < 128;          // the next tile's loads go out before this one's products, where the registers hold them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const LaneAt<T, HD> at(lane);
     const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
     const int id = win_xcd_id(blockIdx.x, gridDim.x);
     const int split = id % p.nsplit, rest = id / p.nsplit;
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
         for (int u = 0; u < NSUB; ++u) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-            mma_rows<HD>(s[u], lk + u * 32 * G::PB, qf, lane);
+            mma_rows<HD>(s[u], lk + u * 32 * G::PB, qf, at);
         }
         const bool whole = all_live && (key0 + NK <= s0.a || (key0 >= s1.lo && key0 + NK <= s0.hi));
         if (!whole) {
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
                     for (int e = 0; e < 4; ++e) s[u][4 * jj + e] = keep[e] ? s[u][4 * jj + e] * p.drop_scale : 0.f;
                 }
             }
-            mma_cols<HD>(acc, lv + u * 32 * G::PB, s[u], T{}, lane);
+            mma_cols<HD>(acc, lv + u * 32 * G::PB, s[u], at);
         }
     };
 
@@ -306,7 +307,7 @@ WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window
     WinFwdPlan pl;
     const int G = H / Hkv;
     const long rows = (long)nq * G;
-    pl.kw = rows <= 64;
+    pl.kw = win_few_rows((long)B * Hkv, rows);
     const int R = pl.kw ? 32 : 128, BK = pl.kw ? 128 : 64;
     pl.tiles = (int)((rows + R - 1) / R);
     // key tiles that a row tile can see at most
