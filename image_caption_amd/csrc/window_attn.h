@@ -234,20 +234,27 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
         }
 }
 
-// NROWS rows of two strided matrices on their way to LDS; rows past the end arrive as zeros and are not read
+// Rows of a strided matrix from row0 on, as a buffer of which rows nrows.. lie past the end: their loads bring zeros and touch no
+// memory.  (Stride 0 -- one row for all -- has no such end; what is repeated there is a row that is in use.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t win_rows(const char* base, long row0, int nrows, long ss, int row_bytes) {
+    const long bytes = nrows > 0 ? (nrows - 1) * ss + row_bytes : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * ss), 0, (int)(bytes > 0xFFFFFFF0L ? 0xFFFFFFF0u : (unsigned)bytes), 0x00020000);
+}
+
+// NROWS rows of two strided matrices on their way to LDS.  Loads by offset from a bounded buffer: the offsets are the same for
+// every tile, nothing is masked or zeroed by instructions (plain loads under a row test spent 80 instructions a tile on
+// that, and a fifth of the forward's time)
 template <typename T, int HD, int NROWS, int NT> struct TilePair {
     static constexpr int CPR = WinGeo<T, HD>::CPR, U = NROWS * CPR / NT;
     static_assert(NROWS * CPR % NT == 0, "a tile is whole rounds of 16-byte loads");
     u32x4 a[U], b[U];
-    __device__ __forceinline__ void fetch(const char* base0, unsigned ss0, const char* base1, unsigned ss1, int nvalid, int tid) {
+    __device__ __forceinline__ void fetch(const char* base0, long ss0, const char* base1, long ss1, long row0, int nvalid, int tid) {
+        const __amdgpu_buffer_rsrc_t r0 = win_rows(base0, row0, nvalid, ss0, WinGeo<T, HD>::PB), r1 = win_rows(base1, row0, nvalid, ss1, WinGeo<T, HD>::PB);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
-            a[j] = b[j] = u32x4{0, 0, 0, 0};
-            if (row < nvalid) {
-                a[j] = *reinterpret_cast<const u32x4*>(base0 + (unsigned)row * ss0 + ch * 16);
-                b[j] = *reinterpret_cast<const u32x4*>(base1 + (unsigned)row * ss1 + ch * 16);
-            }
+            a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
+            b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
         }
     }
     __device__ __forceinline__ void commit(char* lds0, char* lds1, int tid) const {

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     TilePair<T, HD, BK, NT> tp;
     auto fetch = [&](int idx) {
         const int key0 = tl.at(idx) * BK;
-        tp.fetch(kbase + key0 * kss, (unsigned)kss, vbase + key0 * vss, (unsigned)vss, n - key0, tid);
+        tp.fetch(kbase, kss, vbase, vss, key0, n - key0, tid);
     };
     auto compute = [&](int idx, const char* lk, const char* lv) {
         const int key0 = tl.at(idx) * BK + kw * 32 * NSUB;
