@@ -201,16 +201,21 @@ struct Dec4Args {
     int nsplit; float* part_o; float* part_ml;
 };
 
-// sum / max over the sixteen lanes l & ~15 .. (one key each)
+// sum / max over the sixteen lanes l & ~15 .. (one key each): rotations by 8, 4, 2, 1 lanes inside the rows of sixteen
+template <int N> __device__ __forceinline__ float ror16(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
 __device__ __forceinline__ float sum16(float v) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v += ror16<8>(v);
+    v += ror16<4>(v);
+    v += ror16<2>(v);
+    return v + ror16<1>(v);
 }
 __device__ __forceinline__ float max16(float v) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = fmaxf(v, ror16<8>(v));
+    v = fmaxf(v, ror16<4>(v));
+    v = fmaxf(v, ror16<2>(v));
+    return fmaxf(v, ror16<1>(v));
 }
 // x as NP bf16 numbers that add up to it (NP = 3: all 24 bits)
 template <int NP> __device__ __forceinline__ void split_bf16(float x, bf16_t (&part)[NP]) {
@@ -239,7 +244,8 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
     // visible keys of position n - 1: j < a or lo <= j < n; blocks of 32: 0..ns-1, then ws..
     const int lo = max(0, n - p.window), a = min(p.prefix, n);
     const int ns = (a + 31) >> 5, ws = max(ns, lo >> 5), nt = ns + max(0, ((n + 31) >> 5) - ws);
-    const int t_begin = (int)((long)nt * split / p.nsplit), t_end = (int)((long)nt * (split + 1) / p.nsplit);
+    const int each = nt / p.nsplit, more = nt - each * p.nsplit;                // (the first "more" splits have one block more)
+    const int t_begin = split * each + min(split, more), t_end = t_begin + each + (split < more ? 1 : 0);
     const char* piece = p.cache + bh * k4_piece(p.sm, HD);
     const char* kw = piece + (long)lane * (G::NG * 4);
     const char* vw = piece + k4_v(p.sm, HD) + (long)lane * (G::DW * 4);
@@ -267,13 +273,17 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
     float q16sum[NI][G::NG];
     {
         const int hh = (l16 >> 2) + 4 * (l16 & 3);
-        const T* row = reinterpret_cast<const T*>(p.q) + ((long)b * p.H + h0 + min(hh, nh - 1)) * HD;
+        const T* row = reinterpret_cast<const T*>(p.q) + ((long)b * p.H + h0 + min(hh, nh - 1)) * HD + 8 * g;
+        struct __attribute__((aligned(16))) Eight { T x[8]; } q8[G::NG];
+#pragma unroll
+        for (int t = 0; t < G::NG; ++t) q8[t] = *reinterpret_cast<const Eight*>(row + 32 * t);          // (rows past the group repeat its last)
+        const float on = hh < nh ? 16.f : 0.f;
 #pragma unroll
         for (int t = 0; t < G::NG; ++t) {
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = hh < nh ? 16.f * to_f32<T>(row[32 * t + 8 * g + e]) : 0.f;
+                const float x = on * to_f32<T>(q8[t].x[e]);
                 bf16_t part[NP];
                 split_bf16<NP>(x, part);
 #pragma unroll
