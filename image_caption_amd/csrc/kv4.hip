@@ -153,44 +153,47 @@ struct UnpackArgs {
     const char* cache; long smax, sm; int B, Hkv, n; int start; const int32_t* starts;
     void* k; void* v; long k_bs, k_hs, k_ss, v_bs, v_hs, v_ss;
 };
-// Four channels of K and of V per thread, neighbouring threads on neighbouring channels: whole lines leave.  A word of V holds
-// eight keys of one channel, so it is read for each of them; the 16-32 rows a workgroup works on share their words in its L1.
+// One workgroup: the 32 keys of one block of one (sequence, head), as they are appended.  A thread writes eight channels of a row of
+// K or V, neighbouring threads neighbouring channels, so that whole lines leave.  Eight channels of K are one word and one scale;
+// a word of V holds eight keys of one channel, so the block's words pass through LDS.  Bound by the rows written.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_unpack_kernel(UnpackArgs p) {
     using G = K4<HD>;
-    const int bh = blockIdx.x, b = bh / p.Hkv, h = bh - b * p.Hkv;
+    constexpr int CH = HD / 8, J = 2 * 32 * CH / 256;                        // tasks of a row; of a thread
+    __shared__ __attribute__((aligned(16))) unsigned vl[4 * HD];
+    const int bh = blockIdx.x, b = bh / p.Hkv, h = bh - b * p.Hkv, tid = threadIdx.x;
     const long start = p.starts ? p.starts[b] : p.start;
+    const long s0 = start > 0 ? start : 0, s1 = start + p.n < p.smax ? start + p.n : p.smax;       // rows outside 0..smax-1 are left as they are
     const char* piece = p.cache + bh * k4_piece(p.sm, HD);
-    const long total = (long)p.n * (HD / 4);
-    for (long u = (long)blockIdx.y * 256 + threadIdx.x; u < total; u += (long)gridDim.y * 256) {
-        const int src = (int)(u / (HD / 4)), c4 = (int)(u - (long)src * (HD / 4)) * 4;
-        const long key = start + src;
-        if (key < 0 || key >= p.smax) continue;
-        const int t = c4 >> 5, g = (c4 >> 3) & 3;
-        auto put = [&](void* base, long at, const float (&x)[4]) {
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(reinterpret_cast<T*>(base) + at) = bf16x4{(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3]};
-            else *reinterpret_cast<f32x4*>(reinterpret_cast<T*>(base) + at) = f32x4{x[0], x[1], x[2], x[3]};
-        };
-        float x[4];
-        if (p.k) {
-            const unsigned sw = *reinterpret_cast<const unsigned*>(piece + k4_ks(p.sm, HD) + (key * G::NG + t) * 4);
-            const unsigned w = *reinterpret_cast<const unsigned*>(piece + k4_k_word<HD>((int)key, t, g));
+    for (long block = s0 / 32 + blockIdx.y; block * 32 < s1; block += gridDim.y) {
+        unsigned word[J], scale[J];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = (c4 & 4) + e;
-                x[e] = fmaf(k4_scale(sw), (float)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u), k4_offset(sw));
+        for (int j = 0; j < J; ++j) {
+            const int task = tid + 256 * j, which = task / (32 * CH), row = (task / CH) & 31, ch = task % CH;
+            const int key = (int)block * 32 + row;                           // (inside the piece, which is whole blocks)
+            scale[j] = *reinterpret_cast<const unsigned*>(piece + (which == 0 ? k4_ks(p.sm, HD) : k4_vs(p.sm, HD)) + ((long)key * G::NG + (ch >> 2)) * 4);
+            word[j] = which == 0 ? *reinterpret_cast<const unsigned*>(piece + k4_k_word<HD>(key, ch >> 2, ch & 3)) : 0u;
+        }
+        if (tid < HD) *reinterpret_cast<u32x4*>(vl + 4 * tid) = *reinterpret_cast<const u32x4*>(piece + k4_v(p.sm, HD) + block * (16 * HD) + 16 * tid);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int task = tid + 256 * j, which = task / (32 * CH), row = (task / CH) & 31, ch = task % CH;
+            const long key = block * 32 + row, src = key - start;
+            T* const base = reinterpret_cast<T*>(which == 0 ? p.k : p.v);
+            if (key < s0 || key >= s1 || !base) continue;
+            struct __attribute__((aligned(16))) Eight { T x[8]; } out;
+            const int shift = 4 * ((row & 3) + 4 * (row >> 4)), dt = ch >> 1;
+            const unsigned* vw = vl + ((dt / G::DW) * 64 + ((row & 15) >> 2) * 16 + 8 * (ch & 1)) * G::DW + dt % G::DW;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned level = which == 0 ? (word[j] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u : (vw[e * G::DW] >> shift) & 15u;
+                out.x[e] = from_f32<T>(fmaf(k4_scale(scale[j]), (float)level, k4_offset(scale[j])));
             }
-            put(p.k, (long)b * p.k_bs + (long)h * p.k_hs + src * p.k_ss + c4, x);
+            const long at = which == 0 ? (long)b * p.k_bs + (long)h * p.k_hs + src * p.k_ss : (long)b * p.v_bs + (long)h * p.v_hs + src * p.v_ss;
+            *reinterpret_cast<Eight*>(base + at + 8 * ch) = out;
         }
-        if (p.v) {
-            const unsigned sw = *reinterpret_cast<const unsigned*>(piece + k4_vs(p.sm, HD) + (key * G::NG + t) * 4);
-            const int vg = (int)(key & 15) >> 2, shift = 4 * ((int)(key & 3) + 4 * (int)((key >> 4) & 1));
-            const char* vw = piece + k4_v(p.sm, HD) + k4_v_word<HD>((int)(key >> 5), c4 >> 4, vg, c4 & 15);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[e] = fmaf(k4_scale(sw), (float)((*reinterpret_cast<const unsigned*>(vw + e * (G::DW * 4)) >> shift) & 15u), k4_offset(sw));
-            put(p.v, (long)b * p.v_bs + (long)h * p.v_hs + src * p.v_ss + c4, x);
-        }
+        __syncthreads();
     }
 }
 
@@ -542,8 +545,8 @@ extern "C" int capdec_kv4_unpack(const void* cache, const capdec_kv4_rows* r, in
     const long strides[] = {r->k_bs, r->k_hs, r->k_ss, r->v_bs, r->v_hs, r->v_ss};
     for (long s : strides) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "kv4_unpack: stride %ld (must be a non-negative multiple of %d elements)", s, per16);
     CAPDEC_CHECK(aligned16(r->k) && aligned16(r->v), "kv4_unpack: rows must be 16-byte aligned");
-    const long per = ((long)r->n * (hd / 4) + 255) / 256;
-    const dim3 grid((unsigned)(B * Hkv), (unsigned)(per < 4096 ? per : 4096));
+    const long blocks = starts ? (r->n + 30L) / 32 + 1 : ((long)start + r->n - 1) / 32 - start / 32 + 1;
+    const dim3 grid((unsigned)(B * Hkv), (unsigned)(blocks < 4096 ? blocks : 4096));
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto kfn) { hipLaunchKernelGGL(kfn, grid, dim3(256), 0, st, a); };
     if (r->dtype == CAPDEC_BF16) {
