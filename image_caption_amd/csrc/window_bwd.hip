@@ -48,20 +48,29 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     const int any_a = p.open ? max(s0.a, s1.a) : min(p.prefix, any_hi);
     const int any_end = w_first < p.rows ? max(any_a, any_hi) : 0;
 
-    RowFrag<T, HD> qf, df;
+    RowFrag<T, HD> qf, df, of;
     const long stat = ((long)b * p.H + head) * p.nq + irel;
-    float lse = INFINITY, delta = 0.f;
+    float lse = INFINITY;
     qf.zero();
     df.zero();
+    of.zero();
     if (pos < n) {                     // (a row past its sequence's end holds nothing that may be read into a sum)
-        RowFrag<T, HD> of;
         qf.load(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)head * p.q_hs + (long)irel * p.q_ss, lane);
         df.load(reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)head * p.do_hs + (long)irel * p.do_ss, lane);
         of.load(reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)head * p.o_hs + (long)irel * p.o_ss, lane);
-        delta = df.dot(of);
         lse = p.lse[stat];
-        if (lse == -INFINITY) lse = INFINITY;          // a row that sees nothing: every probability is 0
     }
+    const char* kbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs);
+    const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
+    const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
+    TilePair<T, HD, BK, NT> tp;
+    auto fetch = [&](int idx) {
+        const int key0 = tl.at(idx) * BK;
+        tp.fetch(kbase, kss, vbase, vss, key0, n - key0, tid);
+    };
+    if (tl.nt > 0) fetch(0);           // (on its way before the rows are waited for)
+    if (lse == -INFINITY) lse = INFINITY;              // a row that sees nothing: every probability is 0
+    float delta = df.dot(of);
     delta += __shfl_xor(delta, 32, 64);
     if (kw == 0 && r < p.rows && lane < 32) p.delta[stat] = delta;
 
@@ -71,15 +80,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
 
-    const char* kbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs);
-    const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
-    const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
     const float lsel = lse * WIN_LOG2E;
-    TilePair<T, HD, BK, NT> tp;
-    auto fetch = [&](int idx) {
-        const int key0 = tl.at(idx) * BK;
-        tp.fetch(kbase, kss, vbase, vss, key0, n - key0, tid);
-    };
     auto compute = [&](int idx, const char* lk0, const char* lv0) {
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
@@ -118,7 +119,6 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
         }
     };
     if (tl.nt > 0) {
-        fetch(0);
         if constexpr (NBUF == 2) {
             tp.commit(smem, smem + MAT, tid);
             __syncthreads();
@@ -211,34 +211,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
     const RowBlocks rb = win_row_blocks(p, k0, n);
     const int b_begin = rb.first + (int)((long)rb.count * chunk / nc), b_end = rb.first + (int)((long)rb.count * (chunk + 1) / nc);
 
-    // K's rows stay in LDS and V's in registers: with both in registers the accumulators no longer fit beside them
-    char* lk = smem + 2 * BUF;
-    RowFrag<T, HD> vf;
-    vf.zero();
-    {
-        u32x4 z[KT * CPR / 256];
-#pragma unroll
-        for (int j = 0; j < KT * CPR / 256; ++j) {
-            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
-            z[j] = u32x4{0, 0, 0, 0};
-            if (k0 + row < n)
-                z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)(k0 + row) * p.k_ss + ch * (16 / (int)sizeof(T)));
-        }
-        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
-#pragma unroll
-        for (int j = 0; j < KT * CPR / 256; ++j) {
-            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
-            *reinterpret_cast<u32x4*>(lk + G::at(row, ch)) = z[j];
-        }
-    }
-    vf.landed();
-    const char* lkw = lk + 32 * wave * G::PB;
-    f32x16 dk[G::DT], dv[G::DT];
-#pragma unroll
-    for (int d = 0; d < G::DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-
     // the next block's rows on their way: loaded whatever they hold (rows past the end repeat the last one), and what may not
     // be used -- rows at or past the sequence's end -- put to zero when they reach LDS, so that nothing here waits for a load
     u32x4 fq[U], fd[U];
@@ -260,6 +232,35 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
             f_delta = p.delta[stat0 + (long)g * p.nq + i];
         }
     };
+    // K's rows stay in LDS and V's in registers: with both in registers the accumulators no longer fit beside them
+    char* lk = smem + 2 * BUF;
+    RowFrag<T, HD> vf;
+    vf.zero();
+    {
+        u32x4 z[KT * CPR / 256];
+#pragma unroll
+        for (int j = 0; j < KT * CPR / 256; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            z[j] = u32x4{0, 0, 0, 0};
+            if (k0 + row < n)
+                z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)(k0 + row) * p.k_ss + ch * (16 / (int)sizeof(T)));
+        }
+        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+        if (b_begin < b_end) fetch(b_begin);
+#pragma unroll
+        for (int j = 0; j < KT * CPR / 256; ++j) {
+            const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
+            *reinterpret_cast<u32x4*>(lk + G::at(row, ch)) = z[j];
+        }
+    }
+    vf.landed();
+    const char* lkw = lk + 32 * wave * G::PB;
+    f32x16 dk[G::DT], dv[G::DT];
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+
     auto commit = [&](int blk, char* buf) {
         // rows of a block are in the order of their positions: those before the sequence's end come first
         const int live = min(p.rows, max(0, n - p.q_start) * p.G) - blk * RB;
@@ -337,7 +338,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
         mma_cols<HD>(dk, buf, s, at);
     };
     if (b_begin < b_end) {
-        fetch(b_begin);
         commit(b_begin, smem);
         __syncthreads();
         for (int blk = b_begin; blk < b_end; ++blk) {
