@@ -195,15 +195,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const LaneAt<T, HD> at(lane);
-    const int per_bh = p.kp * p.ncp + (p.ktiles - p.kp) * p.ncn;
-    const int id = win_xcd_id(blockIdx.x, gridDim.x);
-    const int bh = id / per_bh, in = id - bh * per_bh;
-    int tile, chunk, nc, slot;
-    if (in < p.kp * p.ncp) { tile = in / p.ncp; chunk = in - tile * p.ncp; nc = p.ncp; slot = in; }
-    else {
-        const int x = in - p.kp * p.ncp;
+    // the tiles past the prefix come first, the prefix' chunks (shorter, as a rule) fill up behind them; each kind is spread over
+    // the XCDs by itself (in one order over both, one XCD had all the short ones of a head and the other half as many long
+    // ones again as places: 8192 positions 128 wide, 144 steps one after the other where 88 do)
+    const int bhs = p.B * p.Hkv, n_band = bhs * (p.ktiles - p.kp) * p.ncn;
+    int bh, tile, chunk, nc, slot;
+    if ((int)blockIdx.x < n_band) {
+        const int id = win_xcd_id(blockIdx.x, n_band), per = (p.ktiles - p.kp) * p.ncn;
+        bh = id / per;
+        const int x = id - bh * per;
         tile = p.kp + x / p.ncn; chunk = x % p.ncn; nc = p.ncn;
         slot = (p.ncp > 1 ? p.kp * p.ncp : 0) + x;
+    } else {
+        const int id = win_xcd_id(blockIdx.x - n_band, bhs * p.kp * p.ncp), per = p.kp * p.ncp;
+        bh = id / per;
+        slot = id - bh * per;
+        tile = slot / p.ncp; chunk = slot - tile * p.ncp; nc = p.ncp;
     }
     const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
     const int n = win_len(p, b);
