@@ -382,7 +382,15 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
     if (which > 1 || key >= p.S) return;
     const float* at = p.part + ((bh * slots + slot0) * 2 + which) * (long)KT * HD + (long)row * HD + c;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < nc; ++s) v += *reinterpret_cast<const f32x4*>(at + (long)s * 2 * KT * HD);
+    int s = 0;
+    for (; s + 16 <= nc; s += 16) {                                       // sixteen loads at a time, added in order
+        f32x4 x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = *reinterpret_cast<const f32x4*>(at + (long)(s + e) * 2 * KT * HD);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v += x[e];
+    }
+    for (; s < nc; ++s) v += *reinterpret_cast<const f32x4*>(at + (long)s * 2 * KT * HD);
     const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
     T* out = which == 0 ? reinterpret_cast<T*>(p.dk) + (long)b * p.dk_bs + (long)hkv * p.dk_hs + (long)key * p.dk_ss + c
                         : reinterpret_cast<T*>(p.dv) + (long)b * p.dv_bs + (long)hkv * p.dv_hs + (long)key * p.dv_ss + c;
