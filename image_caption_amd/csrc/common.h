@@ -176,6 +176,23 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
     return r;
 }
 
+// sum / max over the sixteen lanes l & ~15 ..: rotations by 8, 4, 2, 1 lanes inside the rows of sixteen
+template <int N> __device__ __forceinline__ float ror16(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float sum16(float v) {
+    v += ror16<8>(v);
+    v += ror16<4>(v);
+    v += ror16<2>(v);
+    return v + ror16<1>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, ror16<8>(v));
+    v = fmaxf(v, ror16<4>(v));
+    v = fmaxf(v, ror16<2>(v));
+    return fmaxf(v, ror16<1>(v));
+}
+
 // ---------------------------------------------------------------- joining attention partials
 // One workgroup of 256 threads per row: o = sum_s e^(m_s - M) O_s / sum_s e^(m_s - M) l_s over nsplit (<= 1024) parts that lie
 // `rows` rows apart, part_o [nsplit][rows][hd] f32 (unnormalised), part_ml [nsplit][rows][2].  The parts are shared out over

@@ -204,22 +204,6 @@ struct Dec4Args {
     int nsplit; float* part_o; float* part_ml;
 };
 
-// sum / max over the sixteen lanes l & ~15 .. (one key each): rotations by 8, 4, 2, 1 lanes inside the rows of sixteen
-template <int N> __device__ __forceinline__ float ror16(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
-}
-__device__ __forceinline__ float sum16(float v) {
-    v += ror16<8>(v);
-    v += ror16<4>(v);
-    v += ror16<2>(v);
-    return v + ror16<1>(v);
-}
-__device__ __forceinline__ float max16(float v) {
-    v = fmaxf(v, ror16<8>(v));
-    v = fmaxf(v, ror16<4>(v));
-    v = fmaxf(v, ror16<2>(v));
-    return fmaxf(v, ror16<1>(v));
-}
 // x as NP bf16 numbers that add up to it (NP = 3: all 24 bits)
 template <int NP> __device__ __forceinline__ void split_bf16(float x, bf16_t (&part)[NP]) {
 #pragma unroll

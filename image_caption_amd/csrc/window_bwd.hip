@@ -184,6 +184,70 @@ __device__ __forceinline__ RowBlocks win_row_blocks(const WinArgs& p, int k0, in
     return {first, (i1 * p.G + RB - 1) / RB - first};
 }
 
+// One step of a wave: RB rows (Q, dO, lse, delta, positions in buf) against its 32 keys (K's rows at lkw, V's in vf): adds to dK and
+// dV and leaves dS [row 8 (e >> 2) + 4 (lane >> 5) + (e & 3)][key lane & 31] in s.  False: none of the rows sees any of the keys.
+template <typename T, int HD, bool DROP>
+__device__ __forceinline__ bool dkv_step(const WinArgs& p, const LaneAt<T, HD>& at, int blk, const char* buf, const char* lkw, const RowFrag<T, HD>& vf, int b,
+                                         int hkv, int n, int kw0, int lane, f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD / 32], f32x16& s) {
+    constexpr int MAT = RB * WinGeo<T, HD>::PB;
+    const int key = kw0 + (lane & 31);
+    const int ra = blk * RB, rz = min(p.rows, ra + RB) - 1;
+    const int pf = p.q_start + win_row_query(p, ra), pl = p.q_start + win_row_query(p, rz);
+    const bool pre = kw0 < p.prefix;
+    const bool band = pl >= kw0 && pf - p.window < kw0 + 31;
+    if (kw0 >= n || !(band || (pre && (p.open || pl >= kw0)))) return false;
+    f32x16 dp;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+    mma_rows_lds<HD>(s, buf, lkw, at);
+    mma_rows<HD>(dp, buf + MAT, vf, at);
+    const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
+    const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * jj);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = sizeof(T) == 2 ? fmaf(s[4 * jj + e], WIN_LOG2E, -lse[e]) : (s[4 * jj + e] - lse[e]) * WIN_LOG2E;
+            s[4 * jj + e] = __builtin_amdgcn_exp2f(x);
+        }
+    }
+    if (!whole) {
+        const int* ps0 = reinterpret_cast<const int*>(st) + 2 * RB;
+        // key <= pos and pos < far, or (a key of the prefix) pos >= near: two intervals of positions per lane
+        const int far = key < n ? key + p.window : 0;                                  // (window <= 2^30, key < 2^28)
+        const int near = key < min(p.prefix, n) ? (p.open ? 0 : key) : 0x7FFFFFFF;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int pos = ps0[8 * jj + e];
+                s[4 * jj + e] = ((pos >= near) | ((pos >= key) & (pos < far))) ? s[4 * jj + e] : 0.f;
+            }
+    }
+    f32x16 pd = s;                                // what multiplies dO: the probabilities after dropout
+    if constexpr (DROP) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int r = min(ra + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), p.rows - 1);
+            const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
+            const uint32_t idx = (uint32_t)((((long)b * p.H + h) * p.S + p.q_start + i) * p.S4) + (uint32_t)key;
+            const float f = dropout_keep(p.drop_k0, p.drop_k1, idx, p.drop_thr) ? p.drop_scale : 0.f;
+            pd[e] *= f;
+            dp[e] *= f;
+        }
+    }
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(st + RB + 8 * jj);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * jj + e] *= dp[4 * jj + e] - delta[e];
+    }
+    mma_cols<HD>(dv, buf + MAT, pd, at);
+    mma_cols<HD>(dk, buf, s, at);
+    return true;
+}
+
 template <typename T, int HD, bool DROP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(WinArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -289,60 +353,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
         }
     };
     auto compute = [&](int blk, const char* buf) {
-        const int ra = blk * RB, rz = min(p.rows, ra + RB) - 1;
-        const int pf = p.q_start + win_row_query(p, ra), pl = p.q_start + win_row_query(p, rz);
-        const bool pre = kw0 < p.prefix;
-        const bool band = pl >= kw0 && pf - p.window < kw0 + 31;
-        if (kw0 >= n || !(band || (pre && (p.open || pl >= kw0)))) return;
-        f32x16 s, dp;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-        mma_rows_lds<HD>(s, buf, lkw, at);
-        mma_rows<HD>(dp, buf + MAT, vf, at);
-        const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
-        const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-            const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * jj);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = sizeof(T) == 2 ? fmaf(s[4 * jj + e], WIN_LOG2E, -lse[e]) : (s[4 * jj + e] - lse[e]) * WIN_LOG2E;
-                s[4 * jj + e] = __builtin_amdgcn_exp2f(x);
-            }
-        }
-        if (!whole) {
-            const int* ps0 = reinterpret_cast<const int*>(st) + 2 * RB;
-            // key <= pos and pos < far, or (a key of the prefix) pos >= near: two intervals of positions per lane
-            const int far = key < n ? key + p.window : 0;                                  // (window <= 2^30, key < 2^28)
-            const int near = key < min(p.prefix, n) ? (p.open ? 0 : key) : 0x7FFFFFFF;
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int pos = ps0[8 * jj + e];
-                    s[4 * jj + e] = ((pos >= near) | ((pos >= key) & (pos < far))) ? s[4 * jj + e] : 0.f;
-                }
-        }
-        f32x16 pd = s;                                // what multiplies dO: the probabilities after dropout
-        if constexpr (DROP) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int r = min(ra + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), p.rows - 1);
-                const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
-                const uint32_t idx = (uint32_t)((((long)b * p.H + h) * p.S + p.q_start + i) * p.S4) + (uint32_t)key;
-                const float f = dropout_keep(p.drop_k0, p.drop_k1, idx, p.drop_thr) ? p.drop_scale : 0.f;
-                pd[e] *= f;
-                dp[e] *= f;
-            }
-        }
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-            const f32x4 delta = *reinterpret_cast<const f32x4*>(st + RB + 8 * jj);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * jj + e] *= dp[4 * jj + e] - delta[e];
-        }
-        mma_cols<HD>(dv, buf + MAT, pd, at);
-        mma_cols<HD>(dk, buf, s, at);
+        f32x16 ds;
+        dkv_step<T, HD, DROP>(p, at, blk, buf, lkw, vf, b, hkv, n, kw0, lane, dk, dv, ds);
     };
     if (b_begin < b_end) {
         commit(b_begin, smem);
@@ -398,6 +410,166 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
     for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(v[e]);
 }
 
+// ------------------------------------------------------------------ all three of short sequences
+// At most 256 keys: one workgroup has them all, eight waves of 32, and goes over the rows once.  A step is dkv_step's; its dS
+// (bf16, as both products take it) also goes to LDS as [key][row], and after every four steps each wave multiplies half of the
+// channels of one of the four blocks' dQ out of it: dQ^T = K^T dS^T with both operands read by columns.  Five products instead of
+// seven, q, k, v and dO read once instead of twice, and delta formed where dO passes by.
+constexpr int SK = 256;
+template <int HD> struct ShortGeo {
+    using G = WinGeo<bf16_t, HD>;
+    static constexpr int MAT = RB * G::PB, BUF = 2 * MAT + 3 * RB * 4, KB = SK * G::PB, DS = SK * RB * 2;
+    static constexpr int LDS = 2 * BUF + KB + 4 * DS;
+};
+template <int HD, bool DROP>
+__global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using T = bf16_t;
+    using G = WinGeo<T, HD>;
+    using L = ShortGeo<HD>;
+    using D = WinGeo<T, RB>;
+    constexpr int CPR = G::CPR, NZ = SK * CPR / 512, NT = HD / 32;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const LaneAt<T, HD> at(lane);
+    const int bh = win_xcd_id(blockIdx.x, gridDim.x);
+    const int b = bh / p.Hkv, hkv = bh - b * p.Hkv;
+    const int n = win_len(p, b);
+    const int kw0 = 32 * wave, key = kw0 + (lane & 31);
+    char* lk = smem + 2 * L::BUF;
+    char* lds_ds = lk + L::KB;
+    const int nblk = (p.rows + RB - 1) / RB;
+
+    // rows on their way: sixteen lanes to a row (of which CPR load), four rows to a wave
+    const int srow = 4 * wave + (lane >> 4), ch = lane & 15;
+    const bool loads = ch < CPR;
+    const int che = (loads ? ch : 0) * 8;
+    u32x4 fq, fd, fo;
+    float f_lse;
+    auto fetch = [&](int blk) {
+        const int r = min(blk * RB + srow, p.rows - 1), i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
+        fq = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i * p.q_ss + che);
+        fd = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.dout) + (long)b * p.do_bs + (long)h * p.do_hs + (long)i * p.do_ss + che);
+        fo = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_ss + che);
+        f_lse = p.lse[((long)b * p.H + h) * p.nq + i];
+    };
+    auto commit = [&](int blk, char* buf) {
+        const bool live = srow < min(p.rows, max(0, n - p.q_start) * p.G) - blk * RB;
+        const u32x4 z = {0, 0, 0, 0};
+        fd = live ? fd : z;
+        fo = live ? fo : z;
+        if (loads) {
+            *reinterpret_cast<u32x4*>(buf + G::at(srow, ch)) = live ? fq : z;
+            *reinterpret_cast<u32x4*>(buf + L::MAT + G::at(srow, ch)) = fd;
+        }
+        const bf16x8 x = __builtin_bit_cast(bf16x8, fd), y = __builtin_bit_cast(bf16x8, fo);
+        float delta = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+        delta = sum16(loads ? delta : 0.f);
+        if (ch == 0) {
+            float* st = reinterpret_cast<float*>(buf + 2 * L::MAT);
+            st[srow] = !live || f_lse == -INFINITY ? INFINITY : f_lse * WIN_LOG2E;
+            st[RB + srow] = delta;
+            reinterpret_cast<int*>(st)[2 * RB + srow] = p.q_start + win_row_query(p, min(blk * RB + srow, p.rows - 1));
+        }
+    };
+
+    RowFrag<T, HD> vf;
+    vf.zero();
+    {
+        u32x4 z[NZ];
+#pragma unroll
+        for (int j = 0; j < NZ; ++j) {
+            const int u = tid + 512 * j, row = u / CPR, c = u - row * CPR;
+            z[j] = u32x4{0, 0, 0, 0};
+            if (row < n) z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)row * p.k_ss + c * 8);
+        }
+        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+        fetch(0);
+#pragma unroll
+        for (int j = 0; j < NZ; ++j) {
+            const int u = tid + 512 * j, row = u / CPR, c = u - row * CPR;
+            *reinterpret_cast<u32x4*>(lk + G::at(row, c)) = z[j];
+        }
+    }
+    vf.landed();
+    f32x16 dk[G::DT], dv[G::DT];
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+
+    commit(0, smem);
+    __syncthreads();
+    for (int blk0 = 0; blk0 < nblk; blk0 += 4) {
+        for (int blk = blk0; blk < min(blk0 + 4, nblk); ++blk) {
+            const bool more = blk + 1 < nblk;
+            if (more) fetch(blk + 1);
+            f32x16 ds;
+            if (!dkv_step<T, HD, DROP>(p, at, blk, smem + (blk & 1) * L::BUF, lk + kw0 * G::PB, vf, b, hkv, n, kw0, lane, dk, dv, ds)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ds[e] = 0.f;
+            }
+            char* to = lds_ds + (blk & 3) * L::DS;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj)
+                *reinterpret_cast<u32x2*>(to + D::at(key, jj) + 8 * (lane >> 5)) =
+                    u32x2{win_pack(ds[4 * jj], ds[4 * jj + 1]), win_pack(ds[4 * jj + 2], ds[4 * jj + 3])};
+            if (more) commit(blk + 1, smem + ((blk + 1) & 1) * L::BUF);
+            __syncthreads();
+        }
+        // 16x16x32 products: lane l holds column l & 15 of either operand and the keys 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3
+        const int rb = wave & 3, half = wave >> 2;
+        if (blk0 + rb < nblk) {
+            const int g = lane >> 4, i16 = lane & 15, krow = 4 * g + (i16 >> 2), sub = (i16 & 3) >> 1, byte = 8 * (i16 & 1);
+            int koff[NT], doff[2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) koff[t] = G::at(krow, half * (CPR / 2) + 2 * t + sub) + byte;
+#pragma unroll
+            for (int rh = 0; rh < 2; ++rh) doff[rh] = D::at(krow, 2 * rh + sub) + byte;
+            f32x4 acc[2][NT];
+#pragma unroll
+            for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[rh][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            auto col = [](const char* at0, int pb) {
+                const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at0));
+                const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, at0 + 16 * pb));
+                return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            const int kb_end = min(8, (n + 31) >> 5);                        // (keys past the end are zero in both)
+            for (int kb = 0; kb < kb_end; ++kb) {
+                bf16x8 x[2];
+#pragma unroll
+                for (int rh = 0; rh < 2; ++rh) x[rh] = col(lds_ds + rb * L::DS + kb * 32 * D::PB + doff[rh], D::PB);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const bf16x8 kc = col(lk + kb * 32 * G::PB + koff[t], G::PB);
+#pragma unroll
+                    for (int rh = 0; rh < 2; ++rh) acc[rh][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, x[rh], acc[rh][t], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int rh = 0; rh < 2; ++rh) {
+                const int r = (blk0 + rb) * RB + 16 * rh + i16;
+                if (r >= p.rows) continue;
+                const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
+                T* out = reinterpret_cast<T*>(p.dq) + (long)b * p.dq_bs + (long)h * p.dq_hs + (long)i * p.dq_ss + half * (HD / 2) + 4 * g;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    *reinterpret_cast<u32x2*>(out + 16 * t) = u32x2{win_pack(acc[rh][t][0] * p.dq_scale, acc[rh][t][1] * p.dq_scale),
+                                                                    win_pack(acc[rh][t][2] * p.dq_scale, acc[rh][t][3] * p.dq_scale)};
+            }
+        }
+        if (blk0 + 4 < nblk) __syncthreads();                               // the next step writes dS where this one was read
+    }
+    const bool ok = key < p.S;
+    const int ks = min(key, p.S - 1);
+    store_rows<HD>(dk, 1.f, reinterpret_cast<T*>(p.dk) + (long)b * p.dk_bs + (long)hkv * p.dk_hs + (long)ks * p.dk_ss, ok, lane);
+    store_rows<HD>(dv, 1.f, reinterpret_cast<T*>(p.dv) + (long)b * p.dv_bs + (long)hkv * p.dv_hs + (long)ks * p.dv_ss, ok, lane);
+}
+
 // ------------------------------------------------------------------ launch
 struct BwdPlan { int ktiles, kp, ncp, ncn; long part_floats; };
 BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix) {
@@ -427,10 +599,22 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
     return pl;
 }
 
+bool win_bwd_short(long bh, int S) { return S > 128 && S <= SK && bh >= 128; }
+
 template <typename T, int HD, bool DROP>
 int bwd_go(WinArgs& a, hipStream_t st) {
     using G = WinGeo<T, HD>;
     const long bh = (long)a.B * a.Hkv;
+    if constexpr (sizeof(T) == 2 && HD <= 96) {
+        if (win_bwd_short(bh, a.S)) {
+            auto kfn = win_bwd_short_kernel<HD, DROP>;
+            static_assert(ShortGeo<HD>::LDS <= 160 * 1024, "LDS of a CU");
+            ensure_dynamic_lds((const void*)kfn, ShortGeo<HD>::LDS);
+            hipLaunchKernelGGL(kfn, dim3((unsigned)bh), dim3(512), ShortGeo<HD>::LDS, st, a);
+            CAPDEC_LAUNCH_CHECK();
+            return CAPDEC_OK;
+        }
+    }
     {
         const bool kw = win_few_rows(bh, a.rows);
         constexpr int NS = sizeof(T) == 2 ? 2 : 1;

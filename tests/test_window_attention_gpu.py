@@ -174,6 +174,50 @@ def test_prefix_gradients_from_many_rows(dtype):
         wo.assert_within(got, w, bd, what)
 
 
+# many short sequences: dQ, dK and dV from one kernel
+SHORT = [
+    (20, 8, 8, 229, 229, 96, 16, 197, True),
+    (16, 16, 8, 256, 256, 64, 0, 0, False),                        # two heads to a K/V head, every row block full
+    (64, 6, 2, 131, 40, 32, 10, 2, False),                         # last rows only, three heads to a K/V head
+    (130, 1, 1, 200, 1, 96, 0, 7, False),                          # one row
+    (33, 20, 4, 160, 160, 64, 31, 150, True),                      # more rows than four keys' worth
+    (128, 1, 1, 255, 255, 32, 1, 0, False),                        # each row sees itself
+]
+
+
+@pytest.mark.parametrize("mode", ["plain", "ragged", "dropout"])
+@pytest.mark.parametrize("case", SHORT)
+def test_backward_of_many_short_sequences(case, mode):
+    B, H, Hkv, S, nq, hd, window, prefix, is_open = case
+    print(case, mode, flush=True)
+    q, k, v, dout = make(B, H, Hkv, S, nq, hd, torch.bfloat16, seed=2, packed=nq == S)
+    ns = [S] * B
+    if mode == "ragged":
+        ends = [0, 1, S, S - 1, 31, 32, 33, S - nq, S - nq + 1, 97, 128, 129]
+        ns = [min(S, max(0, ends[b % len(ends)])) for b in range(B)]
+    lens = torch.tensor(ns, dtype=torch.int32, device=DEV) if mode == "ragged" else None
+    kw = dict(window=window, prefix_len=prefix, prefix_open=is_open, q_start=S - nq)
+    keep = None
+    if mode == "dropout":
+        kw["drop"] = ops.dropout_keys(5, 1, 2, 0.3)
+        keep = ops.attn_dropout_mask(kw["drop"], B, H, S, DEV)[:, :, S - nq:].double() / 0.7
+    see = wo.masks(B, S, nq, S - nq, ns, window, prefix, is_open, DEV)
+    o, lse = run_fwd(q, k, v, lens, **kw)
+    oracle = wo.backward(q, k, v, o, lse, dout, see, hd ** -0.5, keep)
+    for b, n in enumerate(ns):                                     # what lies behind the ends may be anything
+        for t, off in ((q, S - nq), (k, 0), (v, 0), (dout, S - nq), (o, S - nq)):
+            t[b, :, max(0, n - off):] = float("nan")
+        lse[b, :, max(0, n - S + nq):] = float("nan")
+    grads = torch.full((B, H, nq, hd), float("nan"), dtype=torch.bfloat16, device=DEV), *torch.full((2, B, S, Hkv, hd), float("nan"), dtype=torch.bfloat16, device=DEV).transpose(2, 3)
+    delta = torch.empty(B, H, nq, device=DEV)
+    ops.attn_window_bwd(q, k, v, o, lse, dout, *grads, delta, lens=lens, dq_scale=hd ** -0.5, **kw)
+    for got, (w, bd), what in zip(grads, oracle, ("dq", "dk", "dv")):
+        wo.assert_within(got, w, bd, what)
+    first = [t.clone() for t in grads]
+    ops.attn_window_bwd(q, k, v, o, lse, dout, *grads, delta, lens=lens, dq_scale=hd ** -0.5, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(first, grads))
+
+
 def test_gradients_against_differences():
     """float32: directional derivatives of sum(o * dout) by central differences of the kernel's own forward, summed in 64 bits."""
     B, H, Hkv, S, hd = 2, 4, 2, 70, 32
