@@ -184,6 +184,55 @@ __device__ __forceinline__ RowBlocks win_row_blocks(const WinArgs& p, int k0, in
     return {first, (i1 * p.G + RB - 1) / RB - first};
 }
 
+// The two pairs of products of a step, S = Q K^T and dP = dO V^T (s, dp), then dV += P^T dO and dK += dS^T Q, with the reads of
+// LDS AH instructions ahead of the matrix instruction that takes them.  (Left to itself the compiler reads every fragment into
+// the same registers and waits for it before each instruction: an LDS latency each, 4 HD / 16 times a step.  2, 3, 4 ahead are
+// alike; the long case 324 -> 313 us, the captioning stack 140 -> 135 us.)
+constexpr int AH = 3;
+template <int HD>
+__device__ __forceinline__ void step_rows(f32x16& s, f32x16& dp, const char* q, const char* d, const char* lkw, const RowFrag<bf16_t, HD>& vf, const LaneAt<bf16_t, HD>& at) {
+    constexpr int N = HD / 16;
+    bf16x8 a[2 * N], k[N];
+    auto read = [&](int i) {
+        a[i] = *reinterpret_cast<const bf16x8*>((i < N ? q : d) + at.row(i % N));
+        if (i < N) k[i] = *reinterpret_cast<const bf16x8*>(lkw + at.row(i));
+    };
+#pragma unroll
+    for (int i = 0; i < AH; ++i) read(i);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        if (i + AH < 2 * N) read(i + AH);
+        __builtin_amdgcn_sched_barrier(0x6);                                // (the vector and scalar units' instructions may pass)
+        if (i < N) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], k[i % N], s, 0, 0, 0);
+        else dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], vf.f[i % N], dp, 0, 0, 0);
+    }
+}
+template <int HD>
+__device__ __forceinline__ void step_cols(f32x16 (&dv)[HD / 32], f32x16 (&dk)[HD / 32], const f32x16& pd, const f32x16& ds, const char* d, const char* q,
+                                          const LaneAt<bf16_t, HD>& at) {
+    constexpr int DT = HD / 32, N = 2 * DT, PB = WinGeo<bf16_t, HD>::PB;
+    bf16x8 a[2 * N], b[4];
+    auto read = [&](int i) {
+        const char* from = (i < N ? d : q) + at.col(i % DT) + 16 * (i / DT % 2) * PB;
+        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from));
+        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + 8 * PB));
+        a[i] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+#pragma unroll
+    for (int i = 0; i < AH; ++i) read(i);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        if (i + AH < 2 * N) read(i + AH);
+        if (i % DT == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[i / DT][e] = (bf16_t)(i < N ? pd : ds)[8 * (i / DT % 2) + e];
+        }
+        __builtin_amdgcn_sched_barrier(0x6);
+        f32x16& acc = (i < N ? dv : dk)[i % DT];
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[i / DT], acc, 0, 0, 0);
+    }
+}
+
 // One step of a wave: RB rows (Q, dO, lse, delta, positions in buf) against its 32 keys (K's rows at lkw, V's in vf): adds to dK and
 // dV and leaves dS [row 8 (e >> 2) + 4 (lane >> 5) + (e & 3)][key lane & 31] in s.  False: none of the rows sees any of the keys.
 template <typename T, int HD, bool DROP>
@@ -199,8 +248,12 @@ __device__ __forceinline__ bool dkv_step(const WinArgs& p, const LaneAt<T, HD>& 
     f32x16 dp;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-    mma_rows_lds<HD>(s, buf, lkw, at);
-    mma_rows<HD>(dp, buf + MAT, vf, at);
+    if constexpr (sizeof(T) == 2) {
+        step_rows<HD>(s, dp, buf, buf + MAT, lkw, vf, at);
+    } else {
+        mma_rows_lds<HD>(s, buf, lkw, at);
+        mma_rows<HD>(dp, buf + MAT, vf, at);
+    }
     const float* st = reinterpret_cast<const float*>(buf + 2 * MAT) + 4 * (lane >> 5);
     const bool whole = kw0 + 32 <= n && ((pf >= kw0 + 31 && pl - p.window < kw0) || (kw0 + 32 <= p.prefix && (p.open || pf >= kw0 + 31)));
 #pragma unroll
@@ -243,8 +296,12 @@ __device__ __forceinline__ bool dkv_step(const WinArgs& p, const LaneAt<T, HD>& 
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * jj + e] *= dp[4 * jj + e] - delta[e];
     }
-    mma_cols<HD>(dv, buf + MAT, pd, at);
-    mma_cols<HD>(dk, buf, s, at);
+    if constexpr (sizeof(T) == 2) {
+        step_cols<HD>(dv, dk, pd, s, buf + MAT, buf, at);
+    } else {
+        mma_cols<HD>(dv, buf + MAT, pd, at);
+        mma_cols<HD>(dk, buf, s, at);
+    }
     return true;
 }
 
@@ -414,7 +471,9 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
 // At most 256 keys: one workgroup has them all, eight waves of 32, and goes over the rows once.  A step is dkv_step's; its dS
 // (bf16, as both products take it) also goes to LDS as [key][row], and after every four steps each wave multiplies half of the
 // channels of one of the four blocks' dQ out of it: dQ^T = K^T dS^T with both operands read by columns.  Five products instead of
-// seven, q, k, v and dO read once instead of twice, and delta formed where dO passes by.
+// seven, q, k, v and dO read once instead of twice, and delta formed where dO passes by.  1024 heads of 229 rows of 96 channels:
+// 134 us against 159 for the two kernels; the 360 MB alone take 77, the rest is the phases of a CU's one workgroup (140 KB of
+// LDS, eight waves of 220 registers) following each other: K and V 26, the last stores 21, dQ 20.
 constexpr int SK = 256;
 template <int HD> struct ShortGeo {
     using G = WinGeo<bf16_t, HD>;
@@ -599,14 +658,22 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
     return pl;
 }
 
-bool win_bwd_short(long bh, int S) { return S > 128 && S <= SK && bh >= 128; }
+// One kernel for short sequences in bf16: where its workgroups, one per K/V head, fill the card or have few rows to go over one
+// after the other.  Measured in us, one kernel against the two (229 keys, all rows | 32 rows; H = Hkv):
+//   96 channels,  16 heads:  26 /  26 |  8 / 14     64 channels,  16 heads:  23 / 23      32 channels,  16 heads: 23 / 17
+//                256 heads:  34 /  44 | 14 / 21                  256 heads:  29 / 37                   256 heads: 26 / 28
+//                512 heads:  65 /  82 | 27 / 35                  512 heads:  54 / 67                   512 heads: 48 / 40
+// (and 64 keys, 512 heads: 19 / 27, 15 / 23, 15 / 15).  With 32 channels the products are too small a part of a step; with 128 the
+// accumulators, V and the fragments no longer fit the registers.
+template <typename T, int HD> constexpr bool HAS_SHORT = sizeof(T) == 2 && (HD == 64 || HD == 96);
+bool win_bwd_short(long bh, long rows, int S) { return S <= SK && (rows <= 256 || bh >= 256); }
 
 template <typename T, int HD, bool DROP>
 int bwd_go(WinArgs& a, hipStream_t st) {
     using G = WinGeo<T, HD>;
     const long bh = (long)a.B * a.Hkv;
-    if constexpr (sizeof(T) == 2 && HD <= 96) {
-        if (win_bwd_short(bh, a.S)) {
+    if constexpr (HAS_SHORT<T, HD>) {
+        if (win_bwd_short(bh, a.rows, a.S)) {
             auto kfn = win_bwd_short_kernel<HD, DROP>;
             static_assert(ShortGeo<HD>::LDS <= 160 * 1024, "LDS of a CU");
             ensure_dynamic_lds((const void*)kfn, ShortGeo<HD>::LDS);

@@ -182,6 +182,10 @@ SHORT = [
     (130, 1, 1, 200, 1, 96, 0, 7, False),                          # one row
     (33, 20, 4, 160, 160, 64, 31, 150, True),                      # more rows than four keys' worth
     (128, 1, 1, 255, 255, 32, 1, 0, False),                        # each row sees itself
+    (64, 6, 2, 131, 40, 64, 10, 2, False),
+    (3, 1, 1, 256, 256, 64, 1, 0, False),
+    (2, 3, 3, 1, 1, 96, 0, 0, False),                              # one token
+    (300, 4, 1, 70, 70, 64, 20, 5, True),                          # 280 rows, more workgroups than CUs
 ]
 
 
