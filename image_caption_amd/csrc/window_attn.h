@@ -189,12 +189,6 @@ template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const ch
 }
 
 // the same with the second operand's rows in LDS as well
-template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, const LaneAt<bf16_t, HD>& at) {
-#pragma unroll
-    for (int s = 0; s < HD / 16; ++s)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(lds + at.row(s)), *reinterpret_cast<const bf16x8*>(rows + at.row(s)),
-                                                      acc, 0, 0, 0);
-}
 template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, const char* lds, const char* rows, const LaneAt<float, HD>& at) {
 #pragma unroll
     for (int s = 0; s < HD / 8; ++s) {
@@ -206,19 +200,25 @@ template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, cons
 
 // p is rounded to bf16 (half a step, 2^-8 of each term) to be an operand: the products' own inputs have no more bits
 template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<bf16_t, HD>& at) {
-    constexpr int PB = WinGeo<bf16_t, HD>::PB;
+    constexpr int PB = WinGeo<bf16_t, HD>::PB, DT = HD / 32, A = 3 < 2 * DT ? 3 : 2 * DT;
+    bf16x8 a[2 * DT], pb[2];
+    auto read = [&](int i) {
+        const char* from = lds + at.col(i % DT) + 16 * (i / DT) * PB;
+        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from));
+        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + 8 * PB));
+        a[i] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        bf16x8 pb;
+    for (int i = 0; i < A; ++i) read(i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pb[e] = (bf16_t)p[8 * c + e];
+    for (int i = 0; i < 2 * DT; ++i) {
+        if (i + A < 2 * DT) read(i + A);
+        if (i % DT == 0) {
 #pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt) {
-            const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, lds + at.col(dt) + (16 * c) * PB));
-            const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, lds + at.col(dt) + (16 * c + 8) * PB));
-            const bf16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb, acc[dt], 0, 0, 0);
+            for (int e = 0; e < 8; ++e) pb[i / DT][e] = (bf16_t)p[8 * (i / DT) + e];
         }
+        __builtin_amdgcn_sched_barrier(0x6);
+        acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], pb[i / DT], acc[i % DT], 0, 0, 0);
     }
 }
 template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<float, HD>& at) {
@@ -232,6 +232,32 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
             const int off = row * G::PB + 4 * h * G::PB + (((8 * dt + (d >> 2)) ^ ((e & 3) << 1 | h)) << 4) + 4 * (d & 3);
             acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(lds + off), p[e], acc[dt], 0, 0, 0);
         }
+}
+
+// Two products of rows one after the other, and columns, with the reads of LDS AH instructions ahead of the matrix instruction
+// that takes them
+constexpr int AH = 3;
+template <int HD>
+__device__ __forceinline__ void mma_rows2(f32x16& s, const char* l0, const RowFrag<bf16_t, HD>& b0, f32x16& t, const char* l1, const RowFrag<bf16_t, HD>& b1,
+                                          const LaneAt<bf16_t, HD>& at) {
+    constexpr int N = HD / 16;
+    bf16x8 a[2 * N];
+    auto read = [&](int i) { a[i] = *reinterpret_cast<const bf16x8*>((i < N ? l0 : l1) + at.row(i % N)); };
+#pragma unroll
+    for (int i = 0; i < AH; ++i) read(i);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        if (i + AH < 2 * N) read(i + AH);
+        __builtin_amdgcn_sched_barrier(0x6);
+        if (i < N) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b0.f[i % N], s, 0, 0, 0);
+        else t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b1.f[i % N], t, 0, 0, 0);
+    }
+}
+template <int HD>
+__device__ __forceinline__ void mma_rows2(f32x16& s, const char* l0, const RowFrag<float, HD>& b0, f32x16& t, const char* l1, const RowFrag<float, HD>& b1,
+                                          const LaneAt<float, HD>& at) {
+    mma_rows<HD>(s, l0, b0, at);
+    mma_rows<HD>(t, l1, b1, at);
 }
 
 // Rows of a strided matrix from row0 on, as a buffer of which rows nrows.. lie past the end: their loads bring zeros and touch no

@@ -91,8 +91,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
             f32x16 s, dp;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-            mma_rows<HD>(s, lk, qf, at);
-            mma_rows<HD>(dp, lv, df, at);
+            mma_rows2<HD>(s, lk, qf, dp, lv, df, at);
             const bool whole = all_live && (key0 + 32 <= s0.a || (key0 >= s1.lo && key0 + 32 <= s0.hi));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -188,7 +187,6 @@ __device__ __forceinline__ RowBlocks win_row_blocks(const WinArgs& p, int k0, in
 // LDS AH instructions ahead of the matrix instruction that takes them.  (Left to itself the compiler reads every fragment into
 // the same registers and waits for it before each instruction: an LDS latency each, 4 HD / 16 times a step.  2, 3, 4 ahead are
 // alike; the long case 324 -> 313 us, the captioning stack 140 -> 135 us.)
-constexpr int AH = 3;
 template <int HD>
 __device__ __forceinline__ void step_rows(f32x16& s, f32x16& dp, const char* q, const char* d, const char* lkw, const RowFrag<bf16_t, HD>& vf, const LaneAt<bf16_t, HD>& at) {
     constexpr int N = HD / 16;

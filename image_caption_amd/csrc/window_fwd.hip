@@ -81,8 +81,9 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
         for (int u = 0; u < NSUB; ++u) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-            mma_rows<HD>(s[u], lk + u * 32 * G::PB, qf, at);
+            if constexpr (NSUB == 1) mma_rows<HD>(s[u], lk + u * 32 * G::PB, qf, at);
         }
+        if constexpr (NSUB == 2) mma_rows2<HD>(s[0], lk, qf, s[1], lk + 32 * G::PB, qf, at);
         const bool whole = all_live && (key0 + NK <= s0.a || (key0 >= s1.lo && key0 + NK <= s0.hi));
         if (!whole) {
 #pragma unroll
