@@ -56,6 +56,15 @@ __device__ __forceinline__ WinSpan win_span(const WinArgs& p, int pos, int n) {
     s.a = live ? min(p.prefix, p.open ? n : s.hi) : 0;
     return s;
 }
+// the keys that some query at pos0..pos1 sees: what lies outside may be anything, and is zero before it meets a probability of 0
+__device__ __forceinline__ WinSpan win_union(const WinArgs& p, int pos0, int pos1, int n) {
+    WinSpan s;
+    const bool live = pos0 < n;
+    s.hi = live ? min(pos1 + 1, n) : 0;
+    s.lo = max(0, pos0 - p.window + 1);
+    s.a = live ? min(p.prefix, p.open ? n : s.hi) : 0;
+    return s;
+}
 // (bitwise, and used in selects only: a branch per element costs more, and a conditional store into a vector's element has
 // come out of the compiler without the store)
 __device__ __forceinline__ bool win_sees(const WinSpan& s, int key) { return (key < s.a) | ((key >= s.lo) & (key < s.hi)); }
@@ -281,6 +290,17 @@ template <typename T, int HD, int NROWS, int NT> struct TilePair {
             const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
             a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
             b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
+        }
+    }
+    // rows before0..from1-1 (relative to the tile) put to zero
+    __device__ __forceinline__ void drop(int before0, int from1, int tid) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int row = (tid + j * NT) / CPR;
+            const u32x4 z = {0, 0, 0, 0};
+            const bool out = (row >= before0) & (row < from1);
+            a[j] = out ? z : a[j];
+            b[j] = out ? z : b[j];
         }
     }
     __device__ __forceinline__ void commit(char* lds0, char* lds1, int tid) const {

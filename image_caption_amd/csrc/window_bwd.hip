@@ -63,10 +63,16 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     const char* kbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs);
     const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
     const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
+    const WinSpan any = win_union(p, q0 + win_row_query(p, r_first), q0 + win_row_query(p, r_end - 1), n);
     TilePair<T, HD, BK, NT> tp;
     auto fetch = [&](int idx) {
         const int key0 = tl.at(idx) * BK;
-        tp.fetch(kbase, kss, vbase, vss, key0, n - key0, tid);
+        tp.fetch(kbase, kss, vbase, vss, key0, max(any.a, any.hi) - key0, tid);
+    };
+    auto commit = [&](int idx, char* lk, char* lv) {
+        const int key0 = tl.at(idx) * BK;
+        if (key0 < any.lo && key0 + BK > any.a) tp.drop(any.a - key0, any.lo - key0, tid);       // (keys between the prefix and the first window)
+        tp.commit(lk, lv, tid);
     };
     if (tl.nt > 0) fetch(0);           // (on its way before the rows are waited for)
     if (lse == -INFINITY) lse = INFINITY;              // a row that sees nothing: every probability is 0
@@ -119,19 +125,19 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     };
     if (tl.nt > 0) {
         if constexpr (NBUF == 2) {
-            tp.commit(smem, smem + MAT, tid);
+            commit(0, smem, smem + MAT);
             __syncthreads();
             for (int idx = 0; idx < tl.nt; ++idx) {
                 const int cur = idx & 1;
                 const bool more = idx + 1 < tl.nt;
                 if (more) fetch(idx + 1);
                 compute(idx, smem + 2 * cur * MAT, smem + (2 * cur + 1) * MAT);
-                if (more) tp.commit(smem + 2 * (cur ^ 1) * MAT, smem + (2 * (cur ^ 1) + 1) * MAT, tid);
+                if (more) commit(idx + 1, smem + 2 * (cur ^ 1) * MAT, smem + (2 * (cur ^ 1) + 1) * MAT);
                 __syncthreads();
             }
         } else {
             for (int idx = 0; idx < tl.nt; ++idx) {
-                tp.commit(smem, smem + MAT, tid);
+                commit(idx, smem, smem + MAT);
                 __syncthreads();
                 if (PRE && idx + 1 < tl.nt) fetch(idx + 1);
                 compute(idx, smem, smem + MAT);
@@ -358,6 +364,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
             f_delta = p.delta[stat0 + (long)g * p.nq + i];
         }
     };
+    const WinSpan any = win_union(p, p.q_start, p.q_start + p.nq - 1, n);
     // K's rows stay in LDS and V's in registers: with both in registers the accumulators no longer fit beside them
     char* lk = smem + 2 * BUF;
     RowFrag<T, HD> vf;
@@ -368,10 +375,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
         for (int j = 0; j < KT * CPR / 256; ++j) {
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
             z[j] = u32x4{0, 0, 0, 0};
-            if (k0 + row < n)
+            if (win_sees(any, k0 + row))
                 z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)(k0 + row) * p.k_ss + ch * (16 / (int)sizeof(T)));
         }
-        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+        if (win_sees(any, key)) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
         if (b_begin < b_end) fetch(b_begin);
 #pragma unroll
         for (int j = 0; j < KT * CPR / 256; ++j) {
@@ -532,6 +539,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         }
     };
 
+    const WinSpan any = win_union(p, p.q_start, p.q_start + p.nq - 1, n);
     RowFrag<T, HD> vf;
     vf.zero();
     {
@@ -540,9 +548,9 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         for (int j = 0; j < NZ; ++j) {
             const int u = tid + 512 * j, row = u / CPR, c = u - row * CPR;
             z[j] = u32x4{0, 0, 0, 0};
-            if (row < n) z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)row * p.k_ss + c * 8);
+            if (win_sees(any, row)) z[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs + (long)row * p.k_ss + c * 8);
         }
-        if (key < n) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
+        if (win_sees(any, key)) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
         fetch(0);
 #pragma unroll
         for (int j = 0; j < NZ; ++j) {

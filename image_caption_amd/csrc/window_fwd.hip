@@ -65,10 +65,16 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     const char* kbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs);
     const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
     const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
+    const WinSpan any = win_union(p, p_first, p_last, n);
     TilePair<T, HD, BK, NT> tp;
     auto fetch = [&](int idx) {
         const int key0 = tl.at(idx) * BK;
-        tp.fetch(kbase, kss, vbase, vss, key0, n - key0, tid);
+        tp.fetch(kbase, kss, vbase, vss, key0, max(any.a, any.hi) - key0, tid);
+    };
+    auto commit = [&](int idx, char* lk, char* lv) {
+        const int key0 = tl.at(idx) * BK;
+        if (key0 < any.lo && key0 + BK > any.a) tp.drop(any.a - key0, any.lo - key0, tid);       // (keys between the prefix and the first window)
+        tp.commit(lk, lv, tid);
     };
     auto compute = [&](int idx, const char* lk, const char* lv) {
         const int key0 = tl.at(idx) * BK + kw * 32 * NSUB;
@@ -135,19 +141,19 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_fwd_
     if (t_begin < t_end) {
         fetch(t_begin);
         if constexpr (NBUF == 2) {
-            tp.commit(smem, smem + MAT, tid);
+            commit(t_begin, smem, smem + MAT);
             __syncthreads();
             for (int idx = t_begin; idx < t_end; ++idx) {
                 const int cur = (idx - t_begin) & 1;
                 const bool more = idx + 1 < t_end;
                 if (more) fetch(idx + 1);
                 compute(idx, smem + 2 * cur * MAT, smem + (2 * cur + 1) * MAT);
-                if (more) tp.commit(smem + 2 * (cur ^ 1) * MAT, smem + (2 * (cur ^ 1) + 1) * MAT, tid);
+                if (more) commit(idx + 1, smem + 2 * (cur ^ 1) * MAT, smem + (2 * (cur ^ 1) + 1) * MAT);
                 __syncthreads();
             }
         } else {
             for (int idx = t_begin; idx < t_end; ++idx) {
-                tp.commit(smem, smem + MAT, tid);
+                commit(idx, smem, smem + MAT);
                 __syncthreads();
                 if (PRE && idx + 1 < t_end) fetch(idx + 1);
                 compute(idx, smem, smem + MAT);

@@ -243,8 +243,8 @@ int capdec_attn_decode(const void* q, const void* kv_cache, void* o, int dtype,
  * (elements; rows 16-byte aligned, strides non-negative multiples of 16 bytes); q carries the hd^-0.5 scale.  Hkv divides H:
  * query head h reads K/V head h / (H / Hkv).  hd 32, 64, 96 or 128; S < 2^28; q_start + nq <= S.
  * lens [B] int32 on the DEVICE (NULL: every sequence has S rows): n of each sequence, taken into 0..S; K, V and q rows at or
- * past n are never used, whatever they hold.  A non-finite value in a row that IS visible to some query of a call may
- * reach other queries of its sequence.
+ * past n are never used, whatever they hold, nor are K and V rows that no query of the call sees.  A non-finite value in a
+ * row that is used may reach any result of its sequence and K/V head.
  * lse [B*H*nq] f32 (NULL: not wanted) receives the log-sum-exp the backward needs.
  * workspace: with capdec_attn_window_fwd_workspace(...) bytes (0: none needed) a call of few rows over many keys is cut along
  * the keys; NULL runs it in one piece.  Results do not depend on its contents; calls that overlap in time need their own. */

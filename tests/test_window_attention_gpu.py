@@ -122,6 +122,48 @@ def test_rows_past_the_end_may_hold_anything(dtype, nq):
         assert not res[0][3][b, :, n:].any() and not res[0][4][b, :, n:].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S,q_start,nq,window,prefix,is_open,hd", [
+    (300, 200, 60, 30, 5, False, 64),                              # a gap inside a tile, and keys behind the last query
+    (300, 200, 60, 30, 150, True, 128),
+    (300, 100, 1, 10, 0, False, 32),
+    (200, 150, 30, 20, 70, False, 96),                             # the one-kernel backward (bf16)
+    (700, 500, 150, 40, 270, False, 64),
+])
+def test_keys_that_no_query_sees_may_hold_anything(S, q_start, nq, window, prefix, is_open, hd, dtype):
+    B, H, Hkv = 2, 4, 2
+    q, k, v, dout = make(B, H, Hkv, S, nq, hd, dtype)
+    seen = wo.masks(B, S, nq, q_start, [S] * B, window, prefix, is_open, DEV)[0].any(0)
+    assert not seen.all()
+    kw = dict(window=window, prefix_len=prefix, prefix_open=is_open, q_start=q_start)
+    res = []
+    for fill in (0.0, float("nan"), float("inf")):
+        k[:, :, ~seen], v[:, :, ~seen] = fill, -fill
+        for split in (True, False):
+            o, lse = run_fwd(q, k, v, None, split=split, **kw)
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            ops.attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, torch.empty(B, H, nq, device=DEV), **kw)
+            assert not dk[:, :, ~seen].any() and not dv[:, :, ~seen].any()
+            res.append((o, lse, dq, dk, dv))
+    for other in (2, 4):
+        for a, b in zip(res[0] + res[1], res[other] + res[other + 1]):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_past_rows_that_left_the_window(dtype):
+    q, cache, o = torch.randn(2, 4, 64, device=DEV, dtype=dtype), torch.randn(2, 2, 2, 900, 64, device=DEV, dtype=dtype), torch.empty(2, 4, 64, device=DEV, dtype=dtype)
+    lens = torch.tensor([700, 333], dtype=torch.int32, device=DEV)
+    res = []
+    for fill in (0.0, float("nan")):
+        for b, n in enumerate((700, 333)):
+            cache[b, :, :, 10:n - 45] = fill
+            cache[b, :, :, n:] = fill
+        ops.attn_window_decode(q, cache, o, window=45, prefix_len=10, lens=lens)
+        res.append(o.clone())
+    assert torch.isfinite(res[1]).all() and torch.equal(*res)
+
+
 def test_lengths_out_of_range_are_taken_into_it():
     q, k, v, _ = make(2, 2, 2, 40, 40, 32, torch.bfloat16)
     kw = dict(window=7, prefix_len=1, prefix_open=False, q_start=0)
