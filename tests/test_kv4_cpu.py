@@ -67,12 +67,13 @@ def test_attention_refuses():
 
 def test_struct_layout_matches_c(tmp_path):
     src = tmp_path / "sz.c"
-    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "capdec.h"\nint main(void){printf("%zu %zu %zu\\n", sizeof(capdec_kv4_rows),'
-                   'offsetof(capdec_kv4_rows, v_ss), offsetof(capdec_kv4_rows, n));return 0;}\n')
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "capdec.h"\nint main(void){printf("%zu %zu %zu %zu %zu\\n", sizeof(capdec_kv4_rows),'
+                   'offsetof(capdec_kv4_rows, v_ss), offsetof(capdec_kv4_rows, n), sizeof(capdec_decode_kv), offsetof(capdec_decode_kv, prefix_len));return 0;}\n')
     exe = tmp_path / "sz"
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-    assert got == [ctypes.sizeof(_lib.Kv4Rows), _lib.Kv4Rows.v_ss.offset, _lib.Kv4Rows.n.offset]
+    assert got == [ctypes.sizeof(_lib.Kv4Rows), _lib.Kv4Rows.v_ss.offset, _lib.Kv4Rows.n.offset,
+                   ctypes.sizeof(_lib.DecodeKv), _lib.DecodeKv.prefix_len.offset]
 
 
 def test_wrappers_refuse_cpu_tensors():

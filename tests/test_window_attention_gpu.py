@@ -399,6 +399,62 @@ def test_two_streams_at_once():
     assert all(torch.equal(a, b) for a, b in zip(alone, outs))
 
 
+@pytest.mark.parametrize("B,H,S", [(4, 8, 229), (1, 4, 400)])       # one kernel for all three gradients, and two
+def test_backward_in_a_graph_and_on_two_streams(B, H, S):
+    hd, kw = 96, dict(window=20, prefix_len=100, prefix_open=True)
+    size = ops.attn_window_bwd_workspace(B, H, H, S, S, hd, window=20, prefix_len=100)
+    sets = []
+    for seed in (1, 2):
+        q, k, v, dout = make(B, H, H, S, S, hd, torch.bfloat16, seed=seed)
+        o, lse = run_fwd(q, k, v, None, q_start=0, **kw)
+        sets.append(dict(ins=(q, k, v, o, lse, dout), grads=[torch.empty_like(t) for t in (q, k, v)], delta=torch.empty(B, H, S, device=DEV),
+                         ws=torch.empty(size, dtype=torch.uint8, device=DEV)))
+
+    def work(c, grads):
+        ops.attn_window_bwd(*c["ins"], *grads, c["delta"], workspace=c["ws"], **kw)
+
+    alone = []
+    for c in sets:
+        grads = [torch.empty_like(t) for t in c["grads"]]
+        work(c, grads)
+        alone.append(grads)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        work(sets[0], sets[0]["grads"])
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        for t in (*sets[0]["grads"], *sets[1]["grads"]):
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            work(sets[1], sets[1]["grads"])
+        torch.cuda.synchronize()
+        for c, want in zip(sets, alone):
+            assert all(torch.equal(a, b) for a, b in zip(c["grads"], want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S", [100, 300])
+def test_broadcast_inputs(S, dtype):
+    """One row of keys for all positions, one sequence for the whole batch, one gradient for every head: stride 0 along any axis."""
+    B, H, Hkv, hd = 3, 4, 2, 64
+    q, k, v, dout = make(B, H, Hkv, S, S, hd, dtype)
+    kw = dict(window=17, prefix_len=3, prefix_open=False)
+    for qq, kk, vv, dd in ((q[:1].expand_as(q), k[:, :, :1].expand_as(k), v, dout[:, :1].expand_as(dout)),
+                           (q[:, :, :1].expand_as(q), k[:1].expand_as(k), v[:, :1].expand_as(v), dout[:, :, :1].expand_as(dout)),
+                           (q, k[:, :1].expand_as(k), v[:, :, :1].expand_as(v), dout[:1].expand_as(dout))):
+        res = []
+        for args in ((qq, kk, vv, dd), tuple(t.contiguous() for t in (qq, kk, vv, dd))):
+            o, lse = run_fwd(*args[:3], None, q_start=0, **kw)
+            grads = [torch.full((B, h, S, hd), float("nan"), dtype=dtype, device=DEV) for h in (H, Hkv, Hkv)]
+            ops.attn_window_bwd(*args[:3], o, lse, args[3], *grads, torch.empty(B, H, S, device=DEV), **kw)
+            res.append((o, lse, *grads))
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*res))
+
+
 # ------------------------------------------------------------------ refusals of the wrappers
 def test_wrapper_refusals(monkeypatch):
     q, k, v, _ = make(1, 4, 2, 20, 20, 32, torch.bfloat16)
