@@ -23,6 +23,10 @@
 // products instead of one, on matrix cores that are idle most of the time anyway.
 // What bounds it is HBM: 5 bits a value, read once.  Four waves of a workgroup take alternate blocks of 32 keys, each with its next block's
 // loads in flight, and join at the end; few sequences are cut along the keys, joined by kv4_join_kernel.
+//
+// Measured (bf16, us): 4 sequences of up to 131072 rows (32 heads on 8 of 128) 86 = 410 MB at 4.8 TB/s, the vector unit busy for half of it; 256
+// sequences of 229 rows (8 heads of 96) 16 = 57 MB at 3.6 TB/s, two blocks a wave, the rest is starting and joining.  Append of
+// 256 x 198 rows 49 (4.2 TB/s read and written), read-back of them to f32 66 (5.4 TB/s).
 #include "common.h"
 
 namespace {
