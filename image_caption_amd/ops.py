@@ -415,9 +415,11 @@ def attn_window_decode(q, kv_cache, o, *, window, prefix_len=0, length=None, len
 
 
 def _decode_heads(q, o, B, hd):
-    _need(q.is_contiguous() and o.is_contiguous() and q.shape == o.shape and q.dtype == o.dtype, "q and o must be contiguous, of one shape and dtype")
-    _need(q.dim() in (2, 3) and q.shape[0] == B and q[0:1].numel() % hd == 0 and (q.dim() == 2 or q.shape[2] == hd), "q must be [{0}, H, {1}] or [{0}, H * {1}]", B, hd)
-    return q.shape[1] if q.dim() == 3 else q.shape[1] // hd
+    shape = q.shape
+    _need(q.is_contiguous() and o.is_contiguous() and shape == o.shape and q.dtype == o.dtype, "q and o must be contiguous, of one shape and dtype")
+    three = len(shape) == 3
+    _need(shape[0] == B and (shape[2] == hd if three else len(shape) == 2 and shape[1] % hd == 0), "q must be [{0}, H, {1}] or [{0}, H * {1}]", B, hd)
+    return shape[1] if three else shape[1] // hd
 
 
 def kv4_cache(B, Hkv, smax, hd, device) -> torch.Tensor:
