@@ -76,46 +76,21 @@ __device__ __forceinline__ int win_xcd_id(int w, int n) {
     return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (w >> 3);
 }
 
-// Rows in LDS: PB bytes each, no padding, their 16-byte chunks permuted by the row (win_chunk) so that neither kind of read
-// meets itself in a bank: mma_rows reads one chunk of 32 rows (eight rows to a 128-byte phase), mma_cols two neighbouring
-// chunks of four rows.  With a pad of 16 bytes the second kind alone cost 42 % of the LDS cycles.
-//   rows of whole 128 bytes:  chunk ^ f,  f = (row & 3) << 1 | (row >> 2 & 1): all of 0..7 over eight rows, and four different
-//                             pairs over four;
-//   rows of 64 or 192 bytes (bf16, 32 or 96 channels): consecutive rows already lie half a phase apart; the low two bits are
-//                             XORed with the reversed bits of row >> 1.
+// Rows in LDS: PB bytes each, no padding, their 16-byte chunks permuted by the row so that neither kind of read meets itself in
+// one of the 64 banks: mma_rows reads one chunk of 16 consecutive rows at a time (16 lanes of 16 bytes a cycle), mma_cols four
+// chunks of four rows (32 lanes of 8 bytes).  Rows of whole 256, of 128 or of 64 bytes leave groups of GROUP = 16, 8 or 4
+// chunks whose banks come again with the next, the second, the fourth row: a chunk's place in its group is XORed with the
+// row's low four bits reversed, cut to the group.  Sixteen rows then differ in a chunk's place, and four consecutive ones in its
+// upper bits, i.e. in which four chunks.  (Permuted for 32 banks both reads took twice their cycles: the prompt's forward 336 us.)
 template <typename T, int HD> struct WinGeo {
     static constexpr int PB = HD * (int)sizeof(T);
     static constexpr int CPR = PB / 16;                          // 16-byte chunks per row
     static constexpr int DT = HD / 32;
-    static constexpr bool WHOLE = PB % 128 == 0;
+    static constexpr int GROUP = PB % 256 == 0 ? 16 : PB % 128 == 0 ? 8 : 4;
     static __device__ __forceinline__ int mix(int row) {
-        return WHOLE ? (row & 3) << 1 | (row >> 2 & 1) : (row >> 1 & 1) << 1 | (row >> 2 & 1);
+        return ((row & 1) << 3 | (row & 2) << 1 | (row & 4) >> 1 | (row & 8) >> 3) & (GROUP - 1);
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * PB + ((chunk ^ mix(row)) << 4); }
-};
-// byte offsets of what a lane reads for mma_rows (chunk 2 s + (lane >> 5) of row lane & 31): the XOR leaves P addresses, the
-// other steps lie a constant further on
-template <typename T, int HD> struct RowAt {
-    using G = WinGeo<T, HD>;
-    static constexpr int P = G::WHOLE ? 4 : 2;
-    int at[P];
-    __device__ __forceinline__ RowAt(int lane) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) at[i] = G::at(lane & 31, 2 * i + (lane >> 5));
-    }
-    __device__ __forceinline__ int operator()(int s) const { return at[s % P] + (s / P) * (32 * P); }
-};
-// the same for the transposing read of mma_cols: four rows 4 (lane >> 5) .. of columns 16 (lane >> 4 & 1) .. + 15 of tile dt
-template <int HD> struct ColAt {
-    using G = WinGeo<bf16_t, HD>;
-    static constexpr int P = G::WHOLE ? 2 : 1;
-    int at[P];
-    __device__ __forceinline__ ColAt(int lane) {
-        const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
-#pragma unroll
-        for (int t = 0; t < P; ++t) at[t] = G::at(row, 4 * t + 2 * (g & 1) + ((i & 3) >> 1)) + 8 * (i & 1);
-    }
-    __device__ __forceinline__ int operator()(int dt) const { return at[dt % P] + (dt / P) * (64 * P); }
 };
 
 // one row per lane (row = lane & 31; the two halves of the wave hold alternate pieces of it), as mma_rows wants it
@@ -170,17 +145,38 @@ template <int HD> struct RowFrag<float, HD> {
     }
 };
 
-// where a lane reads in a tile: computed once per kernel
-template <typename T, int HD> struct LaneAt;
-template <int HD> struct LaneAt<bf16_t, HD> {
-    RowAt<bf16_t, HD> row;
-    ColAt<HD> col;
-    __device__ __forceinline__ LaneAt(int lane) : row(lane), col(lane) {}
+// Where a lane reads in a tile.  row(s): chunk 2 s + (lane >> 5) of row lane & 31, for mma_rows; col(dt): the transposing read of
+// mma_cols, four rows 4 (lane >> 5) .. of columns 16 (lane >> 4 & 1) .. + 15 of tile dt, and col8(dt) the same eight rows on.
+// XORs of one register each (and one instruction with the tile's address), for sixteen registers that would hold them all.
+template <typename T, int HD> struct RowAt {
+    using G = WinGeo<T, HD>;
+    static constexpr int P = G::GROUP / 2;
+    int r0;
+    __device__ __forceinline__ RowAt(int lane) : r0(G::at(lane & 31, lane >> 5)) {}
+    __device__ __forceinline__ int row(int s) const { return (r0 ^ ((s % P) << 5)) + (s / P) * (32 * P); }
 };
-template <int HD> struct LaneAt<float, HD> {
-    RowAt<float, HD> row;
+// fresh(): the same, of which the compiler may not keep XORs from one tile to the next (it would spill for them)
+template <typename T, int HD> struct LaneAt;
+template <int HD> struct LaneAt<bf16_t, HD> : RowAt<bf16_t, HD> {
+    using G = WinGeo<bf16_t, HD>;
+    static constexpr int P = G::GROUP / 4;
+    int c0;
+    __device__ __forceinline__ LaneAt(int lane) : RowAt<bf16_t, HD>(lane) {
+        const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
+        c0 = G::at(row, 2 * (g & 1) + ((i & 3) >> 1)) + 8 * (i & 1);
+    }
+    __device__ __forceinline__ LaneAt fresh() const {
+        LaneAt x = *this;
+        asm volatile("" : "+v"(x.r0), "+v"(x.c0));
+        return x;
+    }
+    __device__ __forceinline__ int col(int dt) const { return (c0 ^ ((dt % P) << 6)) + (dt / P) * (64 * P); }
+    __device__ __forceinline__ int col8(int dt) const { return (c0 ^ ((dt % P) << 6 | 16)) + (dt / P) * (64 * P) + 8 * G::PB; }
+};
+template <int HD> struct LaneAt<float, HD> : RowAt<float, HD> {
     int lane;
-    __device__ __forceinline__ LaneAt(int lane_) : row(lane_), lane(lane_) {}
+    __device__ __forceinline__ LaneAt(int lane_) : RowAt<float, HD>(lane_), lane(lane_) {}
+    __device__ __forceinline__ LaneAt fresh() const { return *this; }
 };
 
 template <int HD> __device__ __forceinline__ void mma_rows(f32x16& acc, const char* lds, const RowFrag<bf16_t, HD>& b, const LaneAt<bf16_t, HD>& at) {
@@ -212,9 +208,9 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
     constexpr int PB = WinGeo<bf16_t, HD>::PB, DT = HD / 32, A = 3 < 2 * DT ? 3 : 2 * DT;
     bf16x8 a[2 * DT], pb[2];
     auto read = [&](int i) {
-        const char* from = lds + at.col(i % DT) + 16 * (i / DT) * PB;
-        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from));
-        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + 8 * PB));
+        const char* from = lds + 16 * (i / DT) * PB;
+        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + at.col(i % DT)));
+        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + at.col8(i % DT)));
         a[i] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 #pragma unroll
@@ -237,15 +233,15 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
     for (int e = 0; e < 16; ++e)
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
-            const int row = 8 * (e >> 2) + (e & 3);               // + 4 h: of the row, mix() takes bits 0..2 only
-            const int off = row * G::PB + 4 * h * G::PB + (((8 * dt + (d >> 2)) ^ ((e & 3) << 1 | h)) << 4) + 4 * (d & 3);
+            const int row = 8 * (e >> 2) + (e & 3);               // + 4 h
+            const int off = (row + 4 * h) * G::PB + (((8 * dt + (d >> 2)) ^ G::mix(row) ^ h << 1) << 4) + 4 * (d & 3);
             acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(lds + off), p[e], acc[dt], 0, 0, 0);
         }
 }
 
 // Two products of rows one after the other, and columns, with the reads of LDS AH instructions ahead of the matrix instruction
 // that takes them
-constexpr int AH = 3;
+constexpr int AH = 2;
 template <int HD>
 __device__ __forceinline__ void mma_rows2(f32x16& s, const char* l0, const RowFrag<bf16_t, HD>& b0, f32x16& t, const char* l1, const RowFrag<bf16_t, HD>& b1,
                                           const LaneAt<bf16_t, HD>& at) {

@@ -227,9 +227,9 @@ __device__ __forceinline__ void step_cols(f32x16 (&dv)[HD / 32], f32x16 (&dk)[HD
     constexpr int DT = HD / 32, N = 2 * DT, PB = WinGeo<bf16_t, HD>::PB;
     bf16x8 a[2 * N], b[4];
     auto read = [&](int i) {
-        const char* from = (i < N ? d : q) + at.col(i % DT) + 16 * (i / DT % 2) * PB;
-        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from));
-        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + 8 * PB));
+        const char* from = (i < N ? d : q) + 16 * (i / DT % 2) * PB;
+        const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + at.col(i % DT)));
+        const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, from + at.col8(i % DT)));
         a[i] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 #pragma unroll
@@ -250,10 +250,11 @@ __device__ __forceinline__ void step_cols(f32x16 (&dv)[HD / 32], f32x16 (&dk)[HD
 // One step of a wave: RB rows (Q, dO, lse, delta, positions in buf) against its 32 keys (K's rows at lkw, V's in vf): adds to dK and
 // dV and leaves dS [row 8 (e >> 2) + 4 (lane >> 5) + (e & 3)][key lane & 31] in s.  False: none of the rows sees any of the keys.
 template <typename T, int HD, bool DROP>
-__device__ __forceinline__ bool dkv_step(const WinArgs& p, const LaneAt<T, HD>& at, int blk, const char* buf, const char* lkw, const RowFrag<T, HD>& vf, int b,
+__device__ __forceinline__ bool dkv_step(const WinArgs& p, const LaneAt<T, HD>& at0, int blk, const char* buf, const char* lkw, const RowFrag<T, HD>& vf, int b,
                                          int hkv, int n, int kw0, int lane, f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD / 32], f32x16& s) {
     constexpr int MAT = RB * WinGeo<T, HD>::PB;
     const int key = kw0 + (lane & 31);
+    const LaneAt<T, HD> at = at0.fresh();
     const int ra = blk * RB, rz = min(p.rows, ra + RB) - 1;
     const int pf = p.q_start + win_row_query(p, ra), pl = p.q_start + win_row_query(p, rz);
     const bool pre = kw0 < p.prefix;
