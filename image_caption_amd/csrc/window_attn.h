@@ -81,7 +81,8 @@ __device__ __forceinline__ int win_xcd_id(int w, int n) {
 // chunks of four rows (32 lanes of 8 bytes).  Rows of whole 256, of 128 or of 64 bytes leave groups of GROUP = 16, 8 or 4
 // chunks whose banks come again with the next, the second, the fourth row: a chunk's place in its group is XORed with the
 // row's low four bits reversed, cut to the group.  Sixteen rows then differ in a chunk's place, and four consecutive ones in its
-// upper bits, i.e. in which four chunks.  (Permuted for 32 banks both reads took twice their cycles: the prompt's forward 336 us.)
+// upper bits, i.e. in which four chunks.  (Permuted for 32 banks both kinds of read took twice their cycles, 8 and 4: 3 % of the
+// captioning stack's backward, nothing of the prompt's forward -- LDS latency counts there, not its bandwidth.)
 template <typename T, int HD> struct WinGeo {
     static constexpr int PB = HD * (int)sizeof(T);
     static constexpr int CPR = PB / 16;                          // 16-byte chunks per row

@@ -17,9 +17,10 @@
 // seven), which no half step of the output asks for.
 //
 // Measured (bf16, us): 8192 positions, 16 heads on 4 of 128 channels, window 1024: dQ 122, dK / dV 190, join 19, 305-315 in all = 530 TFLOP/s
-// of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time: two waves a SIMD
-// (the accumulators of 64 + 64 registers and V's rows allow no third) wait on LDS, which carries 40 KB a wave and step.
-// Two key blocks a wave with half the LDS traffic and one wave a SIMD: 425.
+// of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time: a step is one chain of
+// LDS reads, products, exponentials, products, LDS writes and a barrier, and only two waves a SIMD are there to fill it (the
+// accumulators of 64 + 64 registers and V's rows allow no third).  Left out in turn: dK and dV's products -52, LDS writes
+// -37, S and dP's products -32, loads from L2 -9, exponentials -5.  Two key blocks a wave at one wave a SIMD: 425.
 #include "window_attn.h"
 
 namespace {
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
 // (bf16, as both products take it) also goes to LDS as [key][row], and after every four steps each wave multiplies half of the
 // channels of one of the four blocks' dQ out of it: dQ^T = K^T dS^T with both operands read by columns.  Five products instead of
 // seven, q, k, v and dO read once instead of twice, and delta formed where dO passes by.  1024 heads of 229 rows of 96 channels:
-// 134 us against 159 for the two kernels; the 360 MB alone take 77, the rest is the phases of a CU's one workgroup (140 KB of
+// 130 us against 159 for the two kernels; the 360 MB alone take 77, the rest is the phases of a CU's one workgroup (140 KB of
 // LDS, eight waves of 220 registers) following each other: K and V 26, the last stores 21, dQ 20.  One workgroup per CU that
 // loads its next head's K and V during dQ measured the same, and so did dQ's reads a block ahead.
 constexpr int SK = 256;
