@@ -15,16 +15,19 @@
 //   two bf16 numbers 1 + level / 16 -- one shift and one and-or for two operands, no conversion.
 //   scales: [key][t] words, scale in the low half, offset in the high half.
 //
-// Attention over it.  With the level as 1 + n/16 and q' = 16 q:  sum_c q n = sum_c q' (1 + n/16) - sum_c q', the correction
+// Attention over it, in bf16.  With the level as 1 + n/16 and q' = 16 q:  sum_c q n = sum_c q' (1 + n/16) - sum_c q', the correction
 // being the product's initial accumulator.  S [head][key] has one key per lane, so a key's scales are that lane's own
-// loads:  s = sum_t scale_t (q . n)_t + offset_t (sum of q over t).  For O, p scale_t 16 becomes the bf16 operand (rounded
-// once, half a step; what is subtracted again is the rounded value), and sum_j (p offset_t - 16 p scale_t) is kept per lane
-// and added at the end.  f32 calls split q' and p scale_t into three bf16 parts, which together are the f32 numbers: three
-// products instead of one, on matrix cores that are idle most of the time anyway.
+// loads:  s = sum_t scale_t (q . n)_t + offset_t (sum of q over t).  For O, p scale_t 16 becomes the bf16 operand r (rounded once, half a
+// step), and what the operand carries beyond p's own weight is taken out around the middle level:
+//     sum_j p (offset + scale n) = sum_j r (1 + n/16)  +  sum_j [ p (offset + 7.5 scale) - r (1 + 7.5/16) ]  up to  (r - 16 p scale) (n - 7.5) / 16,
+// the bracket kept per lane and added at the end (around level 0 the rounding's share was twice as large).
+// In f32 the levels become n - 7.5 instead (more instructions; 1 + n/16 costs the sums 23.5 / 4.6 of their digits), q and
+// p scale_t are split into three bf16 parts, which together are the f32 numbers: three products instead of one, on matrix
+// cores that are idle most of the time anyway.
 // What bounds it is HBM: 5 bits a value, read once.  Four waves of a workgroup take alternate blocks of 32 keys, each with its next block's
 // loads in flight, and join at the end; few sequences are cut along the keys, joined by kv4_join_kernel.
 //
-// Measured (bf16, us): 4 sequences of up to 131072 rows (32 heads on 8 of 128) 86 = 410 MB at 4.8 TB/s, the vector unit busy for half of it; 256
+// Measured (bf16, us): 4 sequences of up to 131072 rows (32 heads on 8 of 128) 85 = 410 MB at 4.8 TB/s, the vector unit busy for half of it; 256
 // sequences of 229 rows (8 heads of 96) 16 = 57 MB at 3.6 TB/s, two blocks a wave, the rest is starting and joining.  Append of
 // 256 x 198 rows 49 (4.2 TB/s read and written), read-back of them to f32 66 (5.4 TB/s).
 #include "common.h"
@@ -56,6 +59,16 @@ template <int N> __device__ __forceinline__ void load_words(unsigned (&w)[N], co
 __device__ __forceinline__ bf16x8 k4_expand(unsigned w) {
     return __builtin_bit_cast(bf16x8, (u32x4{((w << 3) & 0x00780078u) | 0x3F803F80u, ((w >> 1) & 0x00780078u) | 0x3F803F80u,
                                              ((w >> 5) & 0x00780078u) | 0x3F803F80u, ((w >> 9) & 0x00780078u) | 0x3F803F80u}));
+}
+// the same as n - 7.5 (five bits: exact)
+__device__ __forceinline__ bf16x8 k4_centred(unsigned w) {
+    u32x4 out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                                            // k = 2 j in nibble j, k = 2 j + 1 in nibble j + 4
+        const float lo = (float)((w >> (4 * j)) & 15u) - 7.5f, hi = (float)((w >> (4 * j + 16)) & 15u) - 7.5f;
+        out[j] = (__float_as_uint(lo) >> 16) | (__float_as_uint(hi) & 0xFFFF0000u);
+    }
+    return __builtin_bit_cast(bf16x8, out);
 }
 __device__ __forceinline__ float k4_scale(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float k4_offset(unsigned w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -219,7 +232,9 @@ template <int NP> __device__ __forceinline__ void split_bf16(float x, bf16_t (&p
 template <typename T, int HD, int NI>
 __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
     using G = K4<HD>;
-    constexpr int NP = sizeof(T) == 2 ? 1 : 3;
+    constexpr bool WIDE = sizeof(T) == 4;                                    // (f32: centred levels, three parts)
+    constexpr int NP = WIDE ? 3 : 1;
+    constexpr float UNIT = WIDE ? 1.f : 16.f;                                // q' and r per q and p scale
     constexpr int PP = 80;                                                   // bytes per row of P in LDS: 32 bf16 and a pad against bank conflicts
     constexpr int PW = NP * G::NG * 16 * PP;                                 // per wave
     constexpr int PJ = HD + 4;
@@ -259,16 +274,16 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
     int idx = t_begin + wave;
     if (idx < t_end) fetch(cur, idx);
 
-    // q' = 16 q of row l16, channels 32 t + 8 g + e, and the sums of q' and q over each group for rows 4 g + i
+    // q' of row l16, channels 32 t + 8 g + e, and its sums over each group for rows 4 g + i
     bf16x8 qf[NP][G::NG];
-    float q16sum[NI][G::NG];
+    float qsum[NI][G::NG];
     {
         const int hh = (l16 >> 2) + 4 * (l16 & 3);
         const T* row = reinterpret_cast<const T*>(p.q) + ((long)b * p.H + h0 + min(hh, nh - 1)) * HD + 8 * g;
         struct __attribute__((aligned(16))) Eight { T x[8]; } q8[G::NG];
 #pragma unroll
         for (int t = 0; t < G::NG; ++t) q8[t] = *reinterpret_cast<const Eight*>(row + 32 * t);          // (rows past the group repeat its last)
-        const float on = hh < nh ? 16.f : 0.f;
+        const float on = hh < nh ? UNIT : 0.f;
 #pragma unroll
         for (int t = 0; t < G::NG; ++t) {
             float sum = 0.f;
@@ -284,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
 #pragma unroll
-            for (int i = 0; i < NI; ++i) q16sum[i][t] = __shfl(sum, 4 * g + i, 64);
+            for (int i = 0; i < NI; ++i) qsum[i][t] = __shfl(sum, 4 * g + i, 64);
         }
     }
     f32x4 acc[G::DT];
@@ -311,13 +326,17 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
             for (int r = 0; r < NI; ++r) s[i][r] = 0.f;
 #pragma unroll
             for (int t = 0; t < G::NG; ++t) {
-                const bf16x8 kf = k4_expand(cur.k[i][t]);
-                f32x4 x = {-q16sum[0][t], NI > 1 ? -q16sum[NI > 1 ? 1 : 0][t] : 0.f, NI > 2 ? -q16sum[NI > 2 ? 2 : 0][t] : 0.f, NI > 2 ? -q16sum[NI > 2 ? 3 : 0][t] : 0.f};
+                const bf16x8 kf = WIDE ? k4_centred(cur.k[i][t]) : k4_expand(cur.k[i][t]);
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (!WIDE) {
+#pragma unroll
+                    for (int r = 0; r < NI; ++r) x[r] = -qsum[r][t];
+                }
 #pragma unroll
                 for (int c = 0; c < NP; ++c) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[c][t], kf, x, 0, 0, 0);
-                const float sc = k4_scale(cur.ks[i][t]), off = k4_offset(cur.ks[i][t]) * 0.0625f;
+                const float sc = k4_scale(cur.ks[i][t]), off = WIDE ? fmaf(7.5f, sc, k4_offset(cur.ks[i][t])) : k4_offset(cur.ks[i][t]) * 0.0625f;
 #pragma unroll
-                for (int r = 0; r < NI; ++r) s[i][r] += fmaf(sc, x[r], off * q16sum[r][t]);
+                for (int r = 0; r < NI; ++r) s[i][r] += fmaf(sc, x[r], off * qsum[r][t]);
             }
         }
         const bool whole = key0 + 32 <= a || (key0 >= lo && key0 + 32 <= n);
@@ -364,11 +383,10 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
                 bf16_t part[2][NP];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    split_bf16<NP>(16.f * pr[i] * k4_scale(cur.vs[i][t]), part[i]);
-                    float back = 0.f;
-#pragma unroll
-                    for (int c = NP - 1; c >= 0; --c) back += (float)part[i][c];
-                    corr[r][t] += fmaf(pr[i], k4_offset(cur.vs[i][t]), -back);
+                    const float sc = k4_scale(cur.vs[i][t]);
+                    split_bf16<NP>(UNIT * pr[i] * sc, part[i]);
+                    corr[r][t] = fmaf(pr[i], fmaf(7.5f, sc, k4_offset(cur.vs[i][t])), corr[r][t]);
+                    if constexpr (!WIDE) corr[r][t] = fmaf(-1.46875f, (float)part[i][0], corr[r][t]);
                 }
 #pragma unroll
                 for (int c = 0; c < NP; ++c) {
@@ -383,7 +401,8 @@ __global__ __launch_bounds__(256, 2) void kv4_decode_kernel(Dec4Args p) {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
         for (int t = 0; t < G::NG; ++t) {
-            const bf16x8 v0 = k4_expand(cur.v[(2 * t) / G::DW][(2 * t) % G::DW]), v1 = k4_expand(cur.v[(2 * t + 1) / G::DW][(2 * t + 1) % G::DW]);
+            const unsigned w0 = cur.v[(2 * t) / G::DW][(2 * t) % G::DW], w1 = cur.v[(2 * t + 1) / G::DW][(2 * t + 1) % G::DW];
+            const bf16x8 v0 = WIDE ? k4_centred(w0) : k4_expand(w0), v1 = WIDE ? k4_centred(w1) : k4_expand(w1);
 #pragma unroll
             for (int c = 0; c < NP; ++c) {
                 const bf16x8 pf = *reinterpret_cast<const bf16x8*>(pl + ((c * G::NG + t) * 16 + l16) * PP + 16 * g);
