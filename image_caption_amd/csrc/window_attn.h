@@ -276,17 +276,29 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t win_rows(const char* base, lon
 // NROWS rows of two strided matrices on their way to LDS.  Loads by offset from a bounded buffer: the offsets are the same for
 // every tile, nothing is masked or zeroed by instructions (plain loads under a row test spent 80 instructions a tile on
 // that, and a fifth of the forward's time)
-template <typename T, int HD, int NROWS, int NT> struct TilePair {
+// ANEW: its offsets are made from tile to tile, for kernels that would spill for 2 U of them kept (dQ of few rows at 128 channels, 84 -> 70 us
+// at 2 x 8 K/V heads of 8 x 237 rows; the forward is 1 % faster with them kept)
+template <typename T, int HD, int NROWS, int NT, bool ANEW = false> struct TilePair {
     static constexpr int CPR = WinGeo<T, HD>::CPR, U = NROWS * CPR / NT;
     static_assert(NROWS * CPR % NT == 0, "a tile is whole rounds of 16-byte loads");
     u32x4 a[U], b[U];
     __device__ __forceinline__ void fetch(const char* base0, long ss0, const char* base1, long ss1, long row0, int nvalid, int tid) {
         const __amdgpu_buffer_rsrc_t r0 = win_rows(base0, row0, nvalid, ss0, WinGeo<T, HD>::PB), r1 = win_rows(base1, row0, nvalid, ss1, WinGeo<T, HD>::PB);
+        if constexpr (ANEW && NT % CPR == 0) {                              // (load j lies NT / CPR rows on)
+            unsigned o0 = (unsigned)(tid / CPR) * (unsigned)ss0 + tid % CPR * 16, o1 = (unsigned)(tid / CPR) * (unsigned)ss1 + tid % CPR * 16;
+            asm volatile("" : "+v"(o0), "+v"(o1));
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
-            a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
-            b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
+            for (int j = 0; j < U; ++j) {
+                a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, o0 + (unsigned)(j * (NT / CPR)) * (unsigned)ss0, 0, 0);
+                b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, o1 + (unsigned)(j * (NT / CPR)) * (unsigned)ss1, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
+                a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
+                b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
+            }
         }
     }
     // rows before0..from1-1 (relative to the tile) put to zero

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     constexpr bool PRE = KW == 1 || HD < 128;          // the next tile's loads go out before this one's products, where the registers hold them
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const LaneAt<T, HD> at(lane);
+    const LaneAt<T, HD> at0(lane);
     const int qw = KW == 1 ? wave : 0, kw = KW == 1 ? 0 : wave;
     const int id = win_xcd_id(blockIdx.x, gridDim.x);
     const int tile = id % p.tiles, bh = id / p.tiles;
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
     const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
     const WinSpan any = win_union(p, q0 + win_row_query(p, r_first), q0 + win_row_query(p, r_end - 1), n);
-    TilePair<T, HD, BK, NT> tp;
+    TilePair<T, HD, BK, NT, true> tp;
     auto fetch = [&](int idx) {
         const int key0 = tl.at(idx) * BK;
         tp.fetch(kbase, kss, vbase, vss, key0, max(any.a, any.hi) - key0, tid);
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
 
     const float lsel = lse * WIN_LOG2E;
     auto compute = [&](int idx, const char* lk0, const char* lv0) {
+        const LaneAt<T, HD> at = at0.fresh();
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
             const int off = kw * 32 * NSUB + 32 * u, key0 = tl.at(idx) * BK + off;
