@@ -341,8 +341,8 @@ def attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> 
     return _lib.load().capdec_attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
 
 
-def _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written):
-    _on_current_device(q, k, v, o, lens, lse, workspace)
+def _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written, more=()):
+    _on_current_device(q, k, v, o, lens, lse, workspace, *more)
     _need(q.dim() == 4 and k.dim() == 4, "q must be [B, H, nq, hd] and k [B, Hkv, S, hd]")
     shape, dtype = q.shape, q.dtype
     B, H, nq, hd = shape
@@ -381,8 +381,7 @@ def attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, delta, *, window, prefix_
         B, H, nq, hd = q.shape
         workspace = torch.empty(attn_window_bwd_workspace(B, H, k.shape[1], k.shape[2], nq, hd, window=window, prefix_len=prefix_len),
                                 dtype=torch.uint8, device=q.device)
-    fwd = _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, False)
-    _on_current_device(dout, dq, dk, dv, delta)
+    fwd = _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, False, (dout, dq, dk, dv, delta))
     shape, kv, dtype = q.shape, k.shape, q.dtype
     _need(delta.dtype == torch.float32 and delta.numel() == shape[0] * shape[1] * shape[2] and delta.is_contiguous(), "delta must be contiguous float32 scratch of B * H * nq")
     desc = AttnWindowBwdDesc(fwd, ptr(dout), *_bhsd(dout, "dout", shape, dtype), ptr(dq), *_bhsd(dq, "dq", shape, dtype, True),
