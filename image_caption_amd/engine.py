@@ -260,6 +260,8 @@ class DecoderEngine:
             raise ValueError(f"window {self.opt.window} needs mask_mode 'prefix_window' or 'window'")
         if self.opt.kv_cache_bits not in (0, 4):
             raise ValueError("kv_cache_bits must be 0 (the compute dtype) or 4")
+        if (self.opt.kv_cache_bits or self.opt.mask_mode in _WINDOW_MASKS) and geo.hd not in (32, 64, 96, 128):
+            raise ValueError(f"window masks and the 4-bit cache need a head dimension of 32, 64, 96 or 128, not {geo.hd}")
         if self.opt.activation not in _ACTS:
             raise ValueError(f"activation must be one of {sorted(_ACTS)}")
         _lib.load()

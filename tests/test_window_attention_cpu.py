@@ -185,3 +185,11 @@ def test_engine_options_refused():
     for bad in (dict(mask_mode="windows"), dict(window=4), dict(mask_mode="prefix_window", window=-1), dict(kv_cache_bits=8)):
         with pytest.raises(ValueError):
             DecoderEngine(geo, EngineOptions(**bad))
+
+
+def test_engine_refuses_head_dimensions_without_kernels():
+    from image_caption_amd.engine import DecoderEngine, EngineOptions, ModelGeometry
+    for opt in (dict(mask_mode="window", window=3), dict(mask_mode="prefix_window"), dict(kv_cache_bits=4)):
+        with pytest.raises(ValueError, match="head dimension"):
+            DecoderEngine(ModelGeometry(96, 2, 128, 503), EngineOptions(**opt))
+        DecoderEngine(ModelGeometry(64, 2, 128, 503), EngineOptions(**opt))
