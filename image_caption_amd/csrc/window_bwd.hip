@@ -409,7 +409,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
 
     auto commit = [&](int blk, char* buf) {
         // rows of a block are in the order of their positions: those before the sequence's end come first
-        const int live = min(p.rows, max(0, n - p.q_start) * p.G) - blk * RB;
+        // (queries are counted before they are multiplied by the heads: (S - q_start) * G may pass 32 bits, rows = nq * G does not)
+        const int live = min(p.nq, max(0, n - p.q_start)) * p.G - blk * RB;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         f_lse = p.lse[((long)b * p.H + h) * p.nq + i];
     };
     auto commit = [&](int blk, char* buf) {
-        const bool live = srow < min(p.rows, max(0, n - p.q_start) * p.G) - blk * RB;
+        const bool live = srow < min(p.nq, max(0, n - p.q_start)) * p.G - blk * RB;
         const u32x4 z = {0, 0, 0, 0};
         fd = live ? fd : z;
         fo = live ? fo : z;
