@@ -204,8 +204,20 @@ template <int HD> __device__ __forceinline__ void mma_rows_lds(f32x16& acc, cons
     }
 }
 
-// p is rounded to bf16 (half a step, 2^-8 of each term) to be an operand: the products' own inputs have no more bits
-template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<bf16_t, HD>& at) {
+// x + the sum of eight bf16 numbers, in f32
+__device__ __forceinline__ float win_sum8(const bf16x8& b, float x) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
+    x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(b, b, 0, 1), one, x, false);
+    x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(b, b, 2, 3), one, x, false);
+    x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(b, b, 4, 5), one, x, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(b, b, 6, 7), one, x, false);
+}
+
+// p is rounded to bf16 (half a step, 2^-8 of each term) to be an operand: the products' own inputs have no more bits.
+// SUM: sum += this lane's rounded p (half of its row's, the other half lies in lane ^ 32)
+template <int HD, bool SUM = false>
+__device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32], const char* lds, const f32x16& p, const LaneAt<bf16_t, HD>& at, float* sum = nullptr) {
     constexpr int PB = WinGeo<bf16_t, HD>::PB, DT = HD / 32, A = 3 < 2 * DT ? 3 : 2 * DT;
     bf16x8 a[2 * DT], pb[2];
     auto read = [&](int i) {
@@ -222,6 +234,7 @@ template <int HD> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[HD / 32
         if (i % DT == 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) pb[i / DT][e] = (bf16_t)p[8 * (i / DT) + e];
+            if constexpr (SUM) *sum = win_sum8(pb[i / DT], *sum);
         }
         __builtin_amdgcn_sched_barrier(0x6);
         acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], pb[i / DT], acc[i % DT], 0, 0, 0);

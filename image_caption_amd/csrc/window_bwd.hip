@@ -12,9 +12,15 @@
 // that leave f32 partial sums in the workspace, added in order by a third kernel.  At most 256 keys: one kernel for all three.
 //
 // Roundings (bf16): P and dS once, to be operands (half a step of each term, as much as the inputs have); delta is an f32 sum over
-// the bf16 o that the forward wrote, so it carries o's own rounding.  Together the gradients lie 0.0024-0.004 of their size from
-// exact ones, against 0.0017 for their own rounding alone.  With an exact delta -- S and dP a second time, two products of seven --
-// dQ would lie at 0.0026 in place of 0.0031-0.0035 (in 64 bits, rounding by rounding), which no half step of the output asks for.
+// the bf16 o that the forward wrote, so it carries o's own rounding.  Both leave a row of dS with a sum that is not quite 0,
+// and what the keys have in common is multiplied by that sum: with channel offsets of 2 and 8 times the keys' spread dQ was
+// 0.009 and 0.035 of its size off.  In exact numbers the sum is 0 and any c may be taken out of the keys, so
+//     dQ = sum_j dS_j K_j - (sum_j dS_j) c,     the sum over the rounded dS, c the common part of some of the visible keys
+// (KeyMean below): one number a row, a 2-term dot product per two elements of dS.  dQ then lies 0.0024-0.0030 of its size from the exact one
+// whatever the offset, dK 0.0024-0.0025, against 0.0017 for their own rounding alone (cost: captioning stack 123.0 -> 127.6 us, 3 of them the
+// dot products, long case 318 -> 321; the sums by matrix instructions against ones 128.3).  With an exact delta -- S and dP a second time,
+// two products of seven -- it would be 0.0023-0.0026, which no half step of the output asks for.  What V's rows have in common
+// reaches delta through o's rounding and stays: an offset of twice V's spread, and dQ and dK lie at 0.005, eight times, at 0.02.
 //
 // Measured (bf16, us): 8192 positions, 16 heads on 4 of 128 channels, window 1024: dQ 122, dK / dV 190, join 19, 305-315 in all = 530 TFLOP/s
 // of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time: a step is one chain of
@@ -28,7 +34,61 @@ namespace {
 constexpr int KT = 128;              // keys of a dK / dV workgroup: four waves of 32
 constexpr int RB = 32;               // rows per step
 
+// The common part c of the keys, for dQ: the mean of 64 keys from the middle of the longer run of visible ones, in the channels where it
+// stands out of the keys' own spread (five standard errors of that mean: what is below would only be the sample's noise, and an offset
+// of 0.6 spreads costs dQ less than the roundings do).  Fewer than 32 keys say nothing: c = 0.
+// Loads at the start of a workgroup, beside the first tile's; partial sums and squares meet in LDS.
+template <int HD, int NT> struct KeyMean {
+    static constexpr int N = 64, P = HD / 2, RG = NT / P, U = (N + RG - 1) / RG;      // channel pairs of a row, rows at a time, rows of a thread
+    static constexpr int PART = RG * HD * 8, BYTES = PART + HD * 4;
+    unsigned x[U];
+    int m;
+    __device__ __forceinline__ void load(const bf16_t* k, long ss, const WinSpan& any, int tid) {
+        const bool one = any.lo <= any.a, band = !one && any.hi - any.lo >= any.a;
+        const int first = band ? any.lo : 0, len = one ? max(any.a, any.hi) : band ? any.hi - any.lo : any.a;
+        m = min(N, len);
+        const int key0 = first + (len - m) / 2, row = tid / P, pair = tid - row * P;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            x[j] = 0;
+            if (row < RG && row + j * RG < m) x[j] = *reinterpret_cast<const unsigned*>(k + (key0 + row + j * RG) * ss + 2 * pair);
+        }
+    }
+    __device__ __forceinline__ void partial(char* lds, int tid) const {
+        const int row = tid / P, pair = tid - row * P;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};                                      // sum and squares of either channel
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const float lo = __uint_as_float(x[j] << 16), hi = __uint_as_float(x[j] & 0xFFFF0000u);
+            s = f32x4{s[0] + lo, fmaf(lo, lo, s[1]), s[2] + hi, fmaf(hi, hi, s[3])};
+        }
+        if (row < RG) *reinterpret_cast<f32x4*>(lds + (row * HD + 2 * pair) * 8) = s;
+    }
+    // (after a barrier; c may be read after another one)
+    __device__ __forceinline__ void finish(char* lds, int tid) const {
+        if (tid >= HD) return;
+        float s = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < RG; ++j) {
+            const f32x2 y = *reinterpret_cast<const f32x2*>(lds + (j * HD + tid) * 8);
+            s += y[0];
+            s2 += y[1];
+        }
+        const float inv = 1.f / (float)max(m, 1), mean = s * inv, var = fmaxf(fmaf(-mean, mean, s2 * inv), 0.f);
+        *reinterpret_cast<float*>(lds + PART + 4 * tid) = m >= 32 && (float)m * mean * mean > 25.f * var ? mean : 0.f;
+    }
+    static __device__ __forceinline__ f32x4 at(const char* lds, int channel) { return *reinterpret_cast<const f32x4*>(lds + PART + 4 * channel); }
+};
+
 // ------------------------------------------------------------------ dQ (and delta)
+// LDS of dQ's kernel: its tiles (KW: also the join of the four waves' shares), then the common part of the keys
+template <typename T, int HD, int QW, int KW> struct DqLds {
+    using G = WinGeo<T, HD>;
+    static constexpr int BK = 32 * KW * (KW == 1 && sizeof(T) == 2 ? 2 : 1);
+    static constexpr int STAGE = (KW == 1 ? 2 : 1) * 2 * BK * G::PB, JOIN = KW == 1 ? 0 : KW * 32 * (HD + 4) * 4;
+    static constexpr int TILES = STAGE > JOIN ? STAGE : JOIN;
+    static constexpr int BYTES = TILES + (sizeof(T) == 2 ? KeyMean<HD, 64 * QW * KW>::BYTES : 0);
+};
 template <typename T, int HD, int QW, int KW, bool DROP>
 __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_kernel(WinArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -75,6 +135,10 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     const char* vbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs);
     const long kss = p.k_ss * (long)sizeof(T), vss = p.v_ss * (long)sizeof(T);
     const WinSpan any = win_union(p, q0 + win_row_query(p, r_first), q0 + win_row_query(p, r_end - 1), n);
+    constexpr bool CENTRE = sizeof(T) == 2;
+    char* lmean = smem + DqLds<T, HD, QW, KW>::TILES;
+    [[maybe_unused]] KeyMean<HD, NT> mean;
+    [[maybe_unused]] float rsum = 0.f;                 // of this lane's half of its row of dS
     TilePair<T, HD, BK, NT, true> tp;
     auto fetch = [&](int idx) {
         const int key0 = tl.at(idx) * BK;
@@ -85,7 +149,10 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
         if (key0 < any.lo && key0 + BK > any.a) tp.drop(any.a - key0, any.lo - key0, tid);       // (keys between the prefix and the first window)
         tp.commit(lk, lv, tid);
     };
-    if (tl.nt > 0) fetch(0);           // (on its way before the rows are waited for)
+    if (tl.nt > 0) {                   // (on its way before the rows are waited for)
+        fetch(0);
+        if constexpr (CENTRE) mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, any, tid);
+    }
     if (lse == -INFINITY) lse = INFINITY;              // a row that sees nothing: every probability is 0
     float delta = df.dot(of);
     delta += __shfl_xor(delta, 32, 64);
@@ -132,13 +199,16 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
-            mma_cols<HD>(acc, lk, s, at);
+            if constexpr (CENTRE) mma_cols<HD, true>(acc, lk, s, at, &rsum);
+            else mma_cols<HD>(acc, lk, s, at);
         }
     };
     if (tl.nt > 0) {
         if constexpr (NBUF == 2) {
             commit(0, smem, smem + MAT);
+            if constexpr (CENTRE) mean.partial(lmean, tid);
             __syncthreads();
+            if constexpr (CENTRE) mean.finish(lmean, tid);
             for (int idx = 0; idx < tl.nt; ++idx) {
                 const int cur = idx & 1;
                 const bool more = idx + 1 < tl.nt;
@@ -148,6 +218,11 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
                 __syncthreads();
             }
         } else {
+            if constexpr (CENTRE) {
+                mean.partial(lmean, tid);
+                __syncthreads();
+                mean.finish(lmean, tid);
+            }
             for (int idx = 0; idx < tl.nt; ++idx) {
                 commit(idx, smem, smem + MAT);
                 __syncthreads();
@@ -156,6 +231,17 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
                 __syncthreads();
                 if (!PRE && idx + 1 < tl.nt) fetch(idx + 1);
             }
+        }
+        if constexpr (CENTRE) {
+            rsum += __shfl_xor(rsum, 32, 64);
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const f32x4 c = mean.at(lmean, 32 * d + 8 * jj + 4 * (lane >> 5));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[d][4 * jj + e] = fmaf(-rsum, c[e], acc[d][4 * jj + e]);
+                }
         }
     }
     if constexpr (KW == 1) {
@@ -498,7 +584,7 @@ constexpr int SK = 256;
 template <int HD> struct ShortGeo {
     using G = WinGeo<bf16_t, HD>;
     static constexpr int MAT = RB * G::PB, BUF = 2 * MAT + 3 * RB * 4, KB = SK * G::PB, DS = SK * RB * 2;
-    static constexpr int LDS = 2 * BUF + KB + 4 * DS;
+    static constexpr int LDS = 2 * BUF + KB + 4 * DS + KeyMean<HD, 512>::BYTES;
 };
 template <int HD, bool DROP>
 __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
@@ -517,6 +603,8 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
     const int kw0 = 32 * wave, key = kw0 + (lane & 31);
     char* lk = smem + 2 * L::BUF;
     char* lds_ds = lk + L::KB;
+    char* lmean = lds_ds + 4 * L::DS;
+    KeyMean<HD, 512> mean;
     const int nblk = (p.rows + RB - 1) / RB;
 
     // rows on their way: sixteen lanes to a row (of which CPR load), four rows to a wave
@@ -567,6 +655,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         }
         if (win_sees(any, key)) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
         fetch(0);
+        mean.load(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs, p.k_ss, any, tid);
 #pragma unroll
         for (int j = 0; j < NZ; ++j) {
             const int u = tid + 512 * j, row = u / CPR, c = u - row * CPR;
@@ -581,7 +670,9 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
 
     commit(0, smem);
+    mean.partial(lmean, tid);
     __syncthreads();
+    mean.finish(lmean, tid);                                                // (read after the first steps, each of which ends in a barrier)
     for (int blk0 = 0; blk0 < nblk; blk0 += 4) {
         for (int blk = blk0; blk < min(blk0 + 4, nblk); ++blk) {
             const bool more = blk + 1 < nblk;
@@ -609,6 +700,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
 #pragma unroll
             for (int rh = 0; rh < 2; ++rh) doff[rh] = D::at(krow, 2 * rh + sub) + byte;
             f32x4 acc[2][NT];
+            float rsum[2] = {0.f, 0.f};
 #pragma unroll
             for (int rh = 0; rh < 2; ++rh)
 #pragma unroll
@@ -622,7 +714,10 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
             for (int kb = 0; kb < kb_end; ++kb) {
                 bf16x8 x[2];
 #pragma unroll
-                for (int rh = 0; rh < 2; ++rh) x[rh] = col(lds_ds + rb * L::DS + kb * 32 * D::PB + doff[rh], D::PB);
+                for (int rh = 0; rh < 2; ++rh) {
+                    x[rh] = col(lds_ds + rb * L::DS + kb * 32 * D::PB + doff[rh], D::PB);
+                    rsum[rh] = win_sum8(x[rh], rsum[rh]);
+                }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const bf16x8 kc = col(lk + kb * 32 * G::PB + koff[t], G::PB);
@@ -632,6 +727,14 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
             }
 #pragma unroll
             for (int rh = 0; rh < 2; ++rh) {
+                rsum[rh] += __shfl_xor(rsum[rh], 16, 64);
+                rsum[rh] += __shfl_xor(rsum[rh], 32, 64);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const f32x4 c = mean.at(lmean, half * (HD / 2) + 16 * t + 4 * g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[rh][t][e] = fmaf(-rsum[rh], c[e], acc[rh][t][e]);
+                }
                 const int r = (blk0 + rb) * RB + 16 * rh + i16;
                 if (r >= p.rows) continue;
                 const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
@@ -705,16 +808,14 @@ int bwd_go(WinArgs& a, hipStream_t st) {
     }
     {
         const bool kw = win_few_rows(bh, a.rows);
-        constexpr int NS = sizeof(T) == 2 ? 2 : 1;
         a.tiles = (a.rows + (kw ? 31 : 127)) / (kw ? 32 : 128);
         CAPDEC_CHECK(bh * a.tiles < (1L << 31), "attn_window_bwd: grid too large");
         auto go = [&](auto kfn, int lds) {
             if (lds > 64 * 1024) ensure_dynamic_lds((const void*)kfn, lds);
             hipLaunchKernelGGL(kfn, dim3((unsigned)(bh * a.tiles)), dim3(256), lds, st, a);
         };
-        constexpr int lds_q = 4 * 32 * NS * G::PB, lds_t = 2 * 128 * G::PB, lds_j = 4 * 32 * (HD + 4) * 4;
-        if (kw) go(win_dq_kernel<T, HD, 1, 4, DROP>, lds_t > lds_j ? lds_t : lds_j);
-        else go(win_dq_kernel<T, HD, 4, 1, DROP>, lds_q);
+        if (kw) go(win_dq_kernel<T, HD, 1, 4, DROP>, DqLds<T, HD, 1, 4>::BYTES);
+        else go(win_dq_kernel<T, HD, 4, 1, DROP>, DqLds<T, HD, 4, 1>::BYTES);
         CAPDEC_LAUNCH_CHECK();
     }
     const long grid = bh * ((long)a.kp * a.ncp + (long)(a.ktiles - a.kp) * a.ncn);

@@ -29,3 +29,76 @@ def test_backward_of_few_queries_before_very_many_keys():
     for got, (want, bound), what in zip((dq, dk[:, :, :nq], dv[:, :, :nq]), oracle, ("dq", "dk", "dv")):
         wo.assert_within(got, want, bound, what)
     assert not dk[:, :, nq:].any() and not dv[:, :, nq:].any()
+
+
+def run(q, k, v, dout, bwd=True, lens=None, **kw):
+    B, H, nq, hd = q.shape
+    o, lse = torch.full_like(q, float("nan")), torch.full((B, H, nq), float("nan"), device=DEV)
+    size = ops.attn_window_fwd_workspace(B, H, k.shape[1], k.shape[2], nq, hd, window=kw["window"], prefix_len=kw["prefix_len"])
+    ops.attn_window_fwd(q, k, v, o, lse=lse, lens=lens, workspace=torch.empty(size, dtype=torch.uint8, device=DEV), **kw)
+    if not bwd:
+        return o, lse
+    dq, dk, dv = torch.full_like(q, float("nan")), torch.full(k.shape, float("nan"), dtype=k.dtype, device=DEV), torch.full(v.shape, float("nan"), dtype=v.dtype, device=DEV)
+    ops.attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, torch.empty(B, H, nq, device=DEV), lens=lens, **kw)
+    return o, lse, dq, dk, dv
+
+
+# B, H, Hkv, S, nq, hd, window, prefix, open: the one-kernel backward; dQ of many rows and of few; a padded batch of each
+COMMON = [
+    (40, 8, 8, 229, 229, 96, 16, 197, True),
+    (64, 8, 4, 256, 100, 64, 0, 0, False),
+    (4, 16, 4, 900, 900, 128, 200, 4, False),
+    (8, 16, 4, 1100, 1100, 64, 0, 0, False),
+    (16, 8, 4, 700, 700, 32, 90, 130, False),
+    (8, 12, 4, 600, 600, 96, 300, 0, False),
+    (2, 8, 2, 500, 12, 128, 0, 0, False),
+    (3, 4, 4, 400, 50, 64, 100, 3, False),
+    (4, 8, 8, 229, 229, 128, 16, 197, True),
+]
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("offset", [0.0, 0.6, 2.0, 8.0, 50.0])
+@pytest.mark.parametrize("case", COMMON)
+def test_bf16_gradients_where_keys_have_a_common_part(case, offset, ragged):
+    """A common part of a sequence's keys changes no probability, so dQ (a row of dS sums to 0) and dK do not depend on it either.
+    Against gradients in 64 bits with an output that was never rounded.  Of dQ's size in the mean square: its own rounding and dS's
+    0.0017 each (a uniform error of at most half a step, 2^-8 at the lower end of a binade), delta's share of the output's rounding as
+    much at most, in all 0.003; half a step, 2^-8 = 0.0039, is the limit."""
+    B, H, Hkv, S, nq, hd, window, prefix, is_open = case
+    print(case, offset, ragged, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(17)
+
+    def normal(*s):
+        return torch.randn(*s, generator=g, device=DEV)
+
+    q, dout = (normal(B, H, nq, hd) * hd ** -0.5).bfloat16(), normal(B, H, nq, hd).bfloat16()
+    k = (normal(B, Hkv, S, hd) + offset * normal(1, Hkv, 1, hd)).bfloat16()
+    v = (normal(B, Hkv, S, hd) + 0.25 * normal(1, Hkv, 1, hd)).bfloat16()
+    ns = [S - 61 * (b % 4) if ragged else S for b in range(B)]
+    lens = torch.tensor(ns, dtype=torch.int32, device=DEV) if ragged else None
+    _, _, dq, dk, dv = run(q, k, v, dout, lens=lens, window=window, prefix_len=prefix, prefix_open=is_open, q_start=S - nq)
+    see = wo.masks(B, S, nq, S - nq, ns, window, prefix, is_open, DEV)
+    off = torch.zeros(3, dtype=torch.float64, device=DEV)
+    size = torch.zeros(3, dtype=torch.float64, device=DEV)
+    for b in range(0, B, 4):
+        part = slice(b, min(B, b + 4))
+        exact_o, exact_lse, _, _ = wo.forward(q[part], k[part], v[part], see[part])
+        wants = wo.backward(q[part], k[part], v[part], exact_o, exact_lse, dout[part], see[part], 1.0)
+        for i, (got, (want, _)) in enumerate(zip((dq[part], dk[part], dv[part]), wants)):
+            off[i] += (got.double() - want).square().sum()
+            size[i] += want.square().sum()
+    rel = (off / size).sqrt().tolist()
+    print("dq, dk, dv off by", rel, flush=True)
+    assert max(rel) <= 2.0 ** -8, rel
+
+
+def test_keys_that_are_all_alike_get_no_dq():
+    """Every key the same: no query can tell them apart, and dQ is what the roundings leave of 0, not a multiple of the key."""
+    for B, S, hd in ((2, 200, 64), (1, 600, 128)):
+        g = torch.Generator(device=DEV).manual_seed(3)
+        q, dout, v = (torch.randn(B, 4, S, hd, generator=g, device=DEV).bfloat16() for _ in range(3))
+        k = (100 * torch.randn(B, 4, 1, hd, generator=g, device=DEV)).bfloat16().expand(B, 4, S, hd)
+        _, _, dq, _, _ = run(q * hd ** -0.5, k, v, dout, window=0, prefix_len=0)
+        # rows that see 32 keys of their tile or more; the sum of 32-bit products left over, of values up to 100 * hd
+        assert dq[:, :, 128:].abs().max().item() <= 2.0 ** -10
