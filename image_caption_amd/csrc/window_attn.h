@@ -295,22 +295,29 @@ template <typename T, int HD, int NROWS, int NT, bool ANEW = false> struct TileP
     static constexpr int CPR = WinGeo<T, HD>::CPR, U = NROWS * CPR / NT;
     static_assert(NROWS * CPR % NT == 0, "a tile is whole rounds of 16-byte loads");
     u32x4 a[U], b[U];
+    // tiles of 128 rows are two buffers of 64: offsets inside a buffer stay below 2^31 for rows up to 32 MiB apart
+    static constexpr int H = NROWS > 64 ? 2 : 1, UH = U / H, RH = NROWS / H;
+    static_assert(NROWS % H == 0 && RH <= 64 && U % H == 0 && RH * CPR % NT == 0, "a half of a tile is whole rounds of loads too");
     __device__ __forceinline__ void fetch(const char* base0, long ss0, const char* base1, long ss1, long row0, int nvalid, int tid) {
-        const __amdgpu_buffer_rsrc_t r0 = win_rows(base0, row0, nvalid, ss0, WinGeo<T, HD>::PB), r1 = win_rows(base1, row0, nvalid, ss1, WinGeo<T, HD>::PB);
-        if constexpr (ANEW && NT % CPR == 0) {                              // (load j lies NT / CPR rows on)
-            unsigned o0 = (unsigned)(tid / CPR) * (unsigned)ss0 + tid % CPR * 16, o1 = (unsigned)(tid / CPR) * (unsigned)ss1 + tid % CPR * 16;
-            asm volatile("" : "+v"(o0), "+v"(o1));
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, o0 + (unsigned)(j * (NT / CPR)) * (unsigned)ss0, 0, 0);
-                b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, o1 + (unsigned)(j * (NT / CPR)) * (unsigned)ss1, 0, 0);
-            }
-        } else {
+        for (int h = 0; h < H; ++h) {
+            const __amdgpu_buffer_rsrc_t r0 = win_rows(base0, row0 + h * RH, nvalid - h * RH, ss0, WinGeo<T, HD>::PB),
+                                         r1 = win_rows(base1, row0 + h * RH, nvalid - h * RH, ss1, WinGeo<T, HD>::PB);
+            if constexpr (ANEW && NT % CPR == 0) {                          // (load j lies NT / CPR rows on)
+                unsigned o0 = (unsigned)(tid / CPR) * (unsigned)ss0 + tid % CPR * 16, o1 = (unsigned)(tid / CPR) * (unsigned)ss1 + tid % CPR * 16;
+                asm volatile("" : "+v"(o0), "+v"(o1));
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
-                a[j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
-                b[j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
+                for (int j = 0; j < UH; ++j) {
+                    a[h * UH + j] = __builtin_amdgcn_raw_buffer_load_b128(r0, o0 + (unsigned)(j * (NT / CPR)) * (unsigned)ss0, 0, 0);
+                    b[h * UH + j] = __builtin_amdgcn_raw_buffer_load_b128(r1, o1 + (unsigned)(j * (NT / CPR)) * (unsigned)ss1, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < UH; ++j) {
+                    const int u = tid + j * NT, row = u / CPR, ch = u - row * CPR;
+                    a[h * UH + j] = __builtin_amdgcn_raw_buffer_load_b128(r0, (unsigned)row * (unsigned)ss0 + ch * 16, 0, 0);
+                    b[h * UH + j] = __builtin_amdgcn_raw_buffer_load_b128(r1, (unsigned)row * (unsigned)ss1 + ch * 16, 0, 0);
+                }
             }
         }
     }

@@ -291,7 +291,9 @@ int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what) {
     CAPDEC_CHECK(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && aligned16(d->o), "%s: operands must be 16-byte aligned", what);
     const long st[] = {d->q_bs, d->q_hs, d->q_ss, d->k_bs, d->k_hs, d->k_ss, d->v_bs, d->v_hs, d->v_ss, d->o_bs, d->o_hs, d->o_ss};
     for (long s : st) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "%s: stride %ld (must be a non-negative multiple of %d elements)", what, s, per16);
-    CAPDEC_CHECK(128L * d->k_ss * e < (1L << 31) && 128L * d->v_ss * e < (1L << 31), "%s: key rows lie too far apart", what);
+    // (a buffer's 64 rows are addressed by 31 bits)
+    CAPDEC_CHECK(64L * d->k_ss * e < (1L << 31) && 64L * d->v_ss * e < (1L << 31), "%s: key rows lie too far apart (%ld and %ld bytes, 32 MiB or more)", what,
+                 d->k_ss * e, d->v_ss * e);
     memset(&a, 0, sizeof(a));
     a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o;
     a.q_bs = d->q_bs; a.q_hs = d->q_hs; a.q_ss = d->q_ss;

@@ -339,6 +339,13 @@ class DecoderEngine:
     def _window_kw(self, prefix_len):
         return dict(window=self.opt.window, prefix_len=prefix_len, prefix_open=_WINDOW_MASKS[self.opt.mask_mode])
 
+    def _check_window_batch(self, B):
+        """The packed projection's rows of one sequence lie 3 * B * d_model elements apart; the kernels take less than 32 MiB."""
+        row = 3 * self.geo.d_model * (2 if self.cdt == torch.bfloat16 else 4)
+        if B * row >= 1 << 25:
+            raise ValueError(f"batch {B} is too large for mask_mode {self.opt.mask_mode!r} at d_model {self.geo.d_model} in {self.cdt}: "
+                             f"at most {((1 << 25) - 1) // row} sequences per GPU")
+
     def _head_views(self, packed, B, S, parts, q_start=0):
         """[B, H, rows, hd] views of the parts (q, k, v or o) of a packed [S*B, parts*d] matrix; the first from q_start on."""
         t = packed.view(S, B, parts, self.geo.nhead, self.geo.hd)
@@ -447,6 +454,8 @@ class DecoderEngine:
             self.prefix_len = source[2] if len(source) > 2 else 0
         if self.opt.mask_mode in ("prefix_causal", "prefix_window") and self.prefix_len <= 0 and source[0] != "concat":
             raise ValueError(f"{self.opt.mask_mode} masking needs the prefix length")
+        if self.opt.mask_mode in _WINDOW_MASKS:
+            self._check_window_batch(B)
         dev = source[1].device
         M = S * B
         self.generation += 1
@@ -888,6 +897,8 @@ class DecoderEngine:
         if nb > 1 and self.opt.mask_mode != "prefix_causal" and not windowed:
             raise ValueError("KV-cached decoding with stacked blocks is only exact under mask_mode='prefix_causal', 'prefix_window' or 'window'")
         B, P, _ = img.shape
+        if windowed and four:                 # (the prompt then attends over its packed projection)
+            self._check_window_batch(B)
         dev = img.device
         S0, smax = P + 2, P + 1 + max_len
         scale = hd ** -0.5

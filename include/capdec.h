@@ -240,7 +240,7 @@ int capdec_attn_decode(const void* q, const void* kv_cache, void* o, int dtype,
  * visible however far the window has moved; window counts the query's own key, 0 means no limit.  A query that sees
  * nothing -- one at or past its sequence's end -- gives zeros and lse -inf, and no gradient.
  * q/o [B,H,nq,hd] (row r of q is position q_start + r), k/v [B,Hkv,S,hd], all addressed as base + b*bs + h*hs + s*ss + j
- * (elements; rows 16-byte aligned, strides non-negative multiples of 16 bytes); q carries the hd^-0.5 scale.  Hkv divides H:
+ * (elements; rows 16-byte aligned, strides non-negative multiples of 16 bytes, k_ss and v_ss below 32 MiB); q carries the hd^-0.5 scale.  Hkv divides H:
  * query head h reads K/V head h / (H / Hkv).  hd 32, 64, 96 or 128; S < 2^28; q_start + nq <= S.
  * lens [B] int32 on the DEVICE (NULL: every sequence has S rows): n of each sequence, taken into 0..S; K, V and q rows at or
  * past n are never used, whatever they hold, nor are K and V rows that no query of the call sees.  A non-finite value in a

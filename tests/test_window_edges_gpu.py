@@ -102,3 +102,49 @@ def test_keys_that_are_all_alike_get_no_dq():
         _, _, dq, _, _ = run(q * hd ** -0.5, k, v, dout, window=0, prefix_len=0)
         # rows that see 32 keys of their tile or more; the sum of 32-bit products left over, of values up to 100 * hd
         assert dq[:, :, 128:].abs().max().item() <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [32, 96, 128])
+@pytest.mark.parametrize("S,nq,window,prefix", [(150, 150, 40, 3), (150, 9, 0, 0), (260, 260, 100, 130)])
+def test_key_rows_far_apart(S, nq, window, prefix, hd, dtype):
+    """K and V rows almost 32 MiB apart, as a projection of thousands of sequences has them: the bits of the same rows packed."""
+    B, H, Hkv = 1, 4, 2
+    print(S, nq, window, prefix, hd, dtype, flush=True)
+    size = torch.empty(0, dtype=dtype).element_size()
+    row = (1 << 25) // size - 16 // size                                  # elements: 16 bytes below 32 MiB
+    buf = torch.empty((S - 1) * row + 2 * Hkv * hd, dtype=dtype, device=DEV)
+    far = buf.as_strided((B, 2, Hkv, S, hd), (0, Hkv * hd, hd, row, 1))
+    g = torch.Generator(device=DEV).manual_seed(9)
+    near = torch.randn(B, 2, Hkv, S, hd, generator=g, device=DEV).to(dtype)
+    far.copy_(near)
+    q = (torch.randn(B, H, nq, hd, generator=g, device=DEV) * hd ** -0.5).to(dtype)
+    dout = torch.randn(B, H, nq, hd, generator=g, device=DEV).to(dtype)
+    kw = dict(window=window, prefix_len=prefix, q_start=S - nq)
+    for a, b in zip(run(q, far[:, 0], far[:, 1], dout, **kw), run(q, near[:, 0], near[:, 1], dout, **kw)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_key_rows_too_far_apart_are_refused():
+    q = torch.zeros(1, 1, 2, 32, dtype=torch.bfloat16, device=DEV)
+    buf = torch.empty((1 << 24) + 32, dtype=torch.bfloat16, device=DEV)
+    k = buf.as_strided((1, 1, 2, 32), (0, 0, 1 << 24, 1))
+    with pytest.raises(RuntimeError, match="too far apart"):
+        ops.attn_window_fwd(q, k, k, torch.empty_like(q), window=0)
+
+
+@pytest.mark.parametrize("bits", [0, 4])
+def test_engine_refuses_a_batch_before_it_starts(bits):
+    from helpers import TINY
+    import helpers
+    from test_parity_gpu import BF16, make_model
+    sh = TINY
+    model = make_model(sh, helpers.make_state_dict(sh, seed=5), BF16, mask_mode="prefix_window", window=3, kv_cache_bits=bits)
+    B = (1 << 25) // (3 * sh.d * 2) + 1
+    img, sos, cap = (torch.zeros(1, n, sh.d, device=DEV).expand(B, n, sh.d) for n in (sh.P, 1, sh.L))
+    with pytest.raises(ValueError, match=f"at most {B - 1} sequences"):
+        model.caption_loss((img, sos, cap), torch.zeros(1, sh.L, dtype=torch.int64, device=DEV).expand(B, sh.L))
+    if bits:
+        with pytest.raises(ValueError, match=f"at most {B - 1} sequences"):
+            model.generate(img, sos, helpers.make_token_table(sh, seed=6).to(DEV), max_len=2)
+    assert not model.engine._bufs                                         # nothing was allocated for it
