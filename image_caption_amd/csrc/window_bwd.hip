@@ -791,6 +791,9 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
 // accumulators, V and the fragments no longer fit the registers.
 template <typename T, int HD> constexpr bool HAS_SHORT = sizeof(T) == 2 && (HD == 64 || HD == 96);
 bool win_bwd_short(long bh, long rows, int S) { return S <= SK && (rows <= 256 || bh >= 256); }
+bool win_bwd_one_kernel(int dtype, int hd, long bh, long rows, int S) {
+    return dtype == CAPDEC_BF16 && (hd == 64 ? HAS_SHORT<bf16_t, 64> : hd == 96 && HAS_SHORT<bf16_t, 96>) && win_bwd_short(bh, rows, S);
+}
 
 template <typename T, int HD, bool DROP>
 int bwd_go(WinArgs& a, hipStream_t st) {
@@ -861,7 +864,8 @@ extern "C" int capdec_attn_window_bwd(const capdec_attn_window_bwd_desc* d, void
     const int per16 = d->fwd.dtype == CAPDEC_BF16 ? 8 : 4;
     const long strides[] = {d->do_bs, d->do_hs, d->do_ss, d->dq_bs, d->dq_hs, d->dq_ss, d->dk_bs, d->dk_hs, d->dk_ss, d->dv_bs, d->dv_hs, d->dv_ss};
     for (long s : strides) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "attn_window_bwd: stride %ld (must be a non-negative multiple of %d elements)", s, per16);
-    const BwdPlan pl = bwd_plan(a.B, a.H, a.Hkv, a.S, a.nq, d->fwd.hd, d->fwd.window, a.prefix);
+    BwdPlan pl = bwd_plan(a.B, a.H, a.Hkv, a.S, a.nq, d->fwd.hd, d->fwd.window, a.prefix);
+    if (win_bwd_one_kernel(d->fwd.dtype, d->fwd.hd, (long)a.B * a.Hkv, a.rows, a.S)) pl.part_floats = 0;       // (no partial sums there)
     CAPDEC_CHECK((long)a.B * a.Hkv < 65536 || pl.part_floats == 0, "attn_window_bwd: B * Hkv %ld", (long)a.B * a.Hkv);
     if (pl.part_floats > 0) {
         if (!d->fwd.workspace || d->fwd.workspace_bytes < pl.part_floats * 4) {

@@ -266,7 +266,8 @@ int capdec_attn_window_fwd(const capdec_attn_window_desc* desc, void* stream);
 
 /* Backward: fwd as in the forward call (o and lse as it wrote them); dout/dq [B,H,nq,hd], dk/dv [B,Hkv,S,hd] (the sum over
  * the heads that share a K/V head).  Every row of dq, dk and dv is written, zeros where nothing was visible.
- * delta [B*H*nq] f32 scratch.  fwd.workspace: capdec_attn_window_bwd_workspace(...) bytes, required unless that is 0.
+ * delta [B*H*nq] f32 scratch.  fwd.workspace: capdec_attn_window_bwd_workspace(...) bytes, required unless that is 0 (it
+ * covers either dtype; bf16 calls over at most 256 keys that one kernel runs take none).
  * No atomics: the same call gives the same bits.  bf16: P and dS are rounded once to be operands and delta = sum dO o carries
  * o's rounding; dQ is freed of what that and a common part of the keys would make together (0.003 of its size at any offset). */
 typedef struct {

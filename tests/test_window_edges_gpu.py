@@ -148,3 +148,26 @@ def test_engine_refuses_a_batch_before_it_starts(bits):
         with pytest.raises(ValueError, match=f"at most {B - 1} sequences"):
             model.generate(img, sos, helpers.make_token_table(sh, seed=6).to(DEV), max_len=2)
     assert not model.engine._bufs                                         # nothing was allocated for it
+
+
+def test_one_kernel_backward_needs_no_workspace():
+    """Few short heads in bf16: the sizes' workspace is for f32 (partial sums); the one-kernel form neither needs nor touches it."""
+    B, H, S, hd, kw = 1, 3, 256, 64, dict(window=9, prefix_len=5)
+    assert ops.attn_window_bwd_workspace(B, H, H, S, S, hd, **kw) > 0
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v, dout = (torch.randn(B, H, S, hd, generator=g, device=DEV) for _ in range(4))
+    for dtype in (torch.bfloat16, torch.float32):
+        args = [t.to(dtype) for t in (q, k, v)]
+        o, lse = run(*args, None, bwd=False, **kw)
+        res = []
+        for ws in (torch.empty(0, dtype=torch.uint8, device=DEV), None):
+            grads = [torch.full_like(t, float("nan")) for t in args]
+            call = lambda: ops.attn_window_bwd(*args, o, lse, dout.to(dtype), *grads, torch.empty(B, H, S, device=DEV), workspace=ws, **kw)
+            if ws is not None and dtype == torch.float32:
+                with pytest.raises(RuntimeError, match="workspace 0 bytes"):
+                    call()
+            else:
+                call()
+                res.append(grads)
+        if dtype == torch.bfloat16:
+            assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*res))
