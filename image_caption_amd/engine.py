@@ -256,8 +256,8 @@ class DecoderEngine:
             raise ValueError("d_model must be divisible by nhead")
         if self.opt.mask_mode not in _MASKS and self.opt.mask_mode not in _WINDOW_MASKS:
             raise ValueError(f"mask_mode must be one of {sorted(_MASKS) + sorted(_WINDOW_MASKS)}")
-        if self.opt.window < 0 or (self.opt.window and self.opt.mask_mode not in _WINDOW_MASKS):
-            raise ValueError(f"window {self.opt.window} needs mask_mode 'prefix_window' or 'window'")
+        if not 0 <= self.opt.window < 1 << 31 or (self.opt.window and self.opt.mask_mode not in _WINDOW_MASKS):
+            raise ValueError(f"window {self.opt.window} must be in 0..2^31 - 1 and needs mask_mode 'prefix_window' or 'window'")
         if self.opt.kv_cache_bits not in (0, 4):
             raise ValueError("kv_cache_bits must be 0 (the compute dtype) or 4")
         if (self.opt.kv_cache_bits or self.opt.mask_mode in _WINDOW_MASKS) and geo.hd not in (32, 64, 96, 128):

@@ -293,6 +293,13 @@ def _need(cond: bool, what: str, *args):
         raise ValueError(what.format(*args))
 
 
+def _fit32(bits: int):
+    """bits: numbers or-ed together that go to the library as 32-bit ints, where larger ones would lose their upper bits
+    unseen (a prefix of 2^32 would hide everything).  The library itself refuses those below 0."""
+    if bits >> 31 not in (0, -1):
+        raise ValueError("windows, prefixes, positions and lengths must be below 2^31")
+
+
 def _on_current_device(*tensors) -> int:
     """The launch goes to the current device's current stream: a tensor of another device must not reach it."""
     dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
@@ -338,10 +345,12 @@ def _ws(workspace):
 
 def attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> int:
     """Bytes that let attn_window_fwd cut a call of few rows over many keys along the keys (0: it would not)."""
+    _fit32(B | H | Hkv | S | nq | hd | window | prefix_len)
     return _lib.load().capdec_attn_window_fwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
 
 
 def _window_desc(q, k, v, o, window, prefix_len, prefix_open, q_start, lens, drop, lse, workspace, o_written, more=()):
+    _fit32(window | prefix_len | q_start)
     _on_current_device(q, k, v, o, lens, lse, workspace, *more)
     _need(q.dim() == 4 and k.dim() == 4, "q must be [B, H, nq, hd] and k [B, Hkv, S, hd]")
     shape, dtype = q.shape, q.dtype
@@ -369,6 +378,7 @@ def attn_window_fwd(q, k, v, o, *, window, prefix_len=0, prefix_open=False, q_st
 
 
 def attn_window_bwd_workspace(B, H, Hkv, S, nq, hd, *, window, prefix_len=0) -> int:
+    _fit32(B | H | Hkv | S | nq | hd | window | prefix_len)
     return _lib.load().capdec_attn_window_bwd_workspace(B, H, Hkv, S, nq, hd, window, prefix_len)
 
 
@@ -394,12 +404,14 @@ def attn_window_bwd(q, k, v, o, lse, dout, dq, dk, dv, delta, *, window, prefix_
 
 
 def attn_window_decode_workspace(B, H, Hkv, hd, smax, *, window, prefix_len=0) -> int:
+    _fit32(B | H | Hkv | hd | smax | window | prefix_len)
     return _lib.load().capdec_attn_window_decode_workspace(B, H, Hkv, hd, smax, window, prefix_len)
 
 
 def attn_window_decode(q, kv_cache, o, *, window, prefix_len=0, length=None, lens=None, workspace=None):
     """One query per sequence, its last position, over kv_cache [B, Hkv, 2, smax, hd]: q, o [B, H, hd] (or [B, H * hd]).
     length: rows of every sequence (default smax); lens [B] int32 (optional): of each, at most length."""
+    _fit32(window | prefix_len | (length or 0))
     dev = _on_current_device(q, kv_cache, o, lens, workspace)
     _need(kv_cache.dim() == 5 and kv_cache.shape[2] == 2 and kv_cache.is_contiguous(), "kv_cache must be a contiguous [B, Hkv, 2, smax, hd] tensor")
     B, Hkv, _, smax, hd = kv_cache.shape
@@ -423,6 +435,7 @@ def _decode_heads(q, o, B, hd):
 
 def kv4_cache(B, Hkv, smax, hd, device) -> torch.Tensor:
     """An empty cache of smax rows per sequence in 4 bits per value: [B, Hkv, bytes] uint8 (the layout is the library's own)."""
+    _fit32(smax | hd)
     size = _lib.load().capdec_kv4_head_bytes(smax, hd)
     _need(size > 0, "no 4-bit cache of {} rows of {} channels (32, 64, 96 or 128)", smax, hd)
     return torch.zeros(B, Hkv, size, dtype=torch.uint8, device=device)
@@ -445,6 +458,7 @@ def _kv4_rows(k, v, B, Hkv, written=False):
 def kv4_append(k, v, cache, *, smax, start=0, starts=None, counts=None):
     """Quantises the rows k, v [B, Hkv, n, hd] into rows start.. (or starts[b]..) of a kv4_cache; counts[b] (optional): how many
     of the n rows sequence b has.  With starts, rows that would fall outside the cache are dropped."""
+    _fit32(smax | start)
     dev = _on_current_device(k, v, cache, starts, counts)
     _need(k.dim() == 4, "k and v must be [B, Hkv, n, hd]")
     B, Hkv = _kv4_geometry(cache, smax, k.shape[3])
@@ -458,6 +472,7 @@ def kv4_append(k, v, cache, *, smax, start=0, starts=None, counts=None):
 
 def kv4_unpack(cache, k_out, v_out, *, smax, start=0, starts=None):
     """The values that rows start.. (or starts[b]..) of a kv4_cache stand for, into k_out / v_out [B, Hkv, n, hd] (one may be None)."""
+    _fit32(smax | start)
     dev = _on_current_device(cache, k_out, v_out, starts)
     t = k_out if k_out is not None else v_out
     _need(t is not None and t.dim() == 4, "k_out and v_out must be [B, Hkv, n, hd]")
@@ -470,11 +485,13 @@ def kv4_unpack(cache, k_out, v_out, *, smax, start=0, starts=None):
 
 
 def attn_decode_kv4_workspace(B, H, Hkv, hd, smax, *, window=0, prefix_len=0) -> int:
+    _fit32(B | H | Hkv | hd | smax | window | prefix_len)
     return _lib.load().capdec_attn_decode_kv4_workspace(B, H, Hkv, hd, smax, window, prefix_len)
 
 
 def attn_decode_kv4(q, cache, o, *, smax, window=0, prefix_len=0, length=None, lens=None, workspace=None):
     """attn_window_decode over a kv4_cache: q, o [B, H, hd]; every key is visible unless a window is given."""
+    _fit32(smax | window | prefix_len | (length or 0))
     dev = _on_current_device(q, cache, o, lens, workspace)
     _need(q.dim() == 3, "q must be [B, H, hd]")
     hd = q.shape[2]

@@ -1,0 +1,60 @@
+"""Host side of the window-attention and 4-bit-cache calls at the ends of what they allow."""
+import pytest
+import torch
+
+from image_caption_amd import ops
+
+BIG = [1 << 31, 1 << 32, (1 << 32) + 5, 1 << 63, -(1 << 31) - 1]       # 2^32 + 5 would arrive as 5, 2^32 as 0
+
+
+@pytest.mark.parametrize("big", BIG)
+def test_numbers_past_32_bits_are_refused(big):
+    """Before anything else is looked at (the tensors are on the CPU, which is refused later, as a RuntimeError)."""
+    q = torch.zeros(1, 2, 4, 32)
+    c = ops.kv4_cache(1, 2, 8, 32, "cpu")
+    one, lse = q[:, :, 0].contiguous(), torch.zeros(1, 2, 4)
+    kv = torch.zeros(1, 2, 2, 4, 32)
+    calls = [lambda **kw: ops.attn_window_fwd(q, q, q, q, **{"window": 4, **kw}),
+             lambda **kw: ops.attn_window_bwd(q, q, q, q, lse, q, q, q, q, lse, **{"window": 4, **kw}),
+             lambda **kw: ops.attn_window_decode(one, kv, one, **{"window": 4, **kw}),
+             lambda **kw: ops.attn_decode_kv4(one, c, one, **{"smax": 8, **kw})]
+    for call in calls:
+        for name in ("window", "prefix_len"):
+            with pytest.raises(ValueError, match="2\\^31"):
+                call(**{name: big})
+    for call in calls[:2]:
+        with pytest.raises(ValueError, match="2\\^31"):
+            call(q_start=big)
+    for call in calls[2:]:
+        with pytest.raises(ValueError, match="2\\^31"):
+            call(length=big)
+    for call in (lambda **kw: ops.kv4_append(q, q, c, **{"smax": 8, **kw}), lambda **kw: ops.kv4_unpack(c, q, q, **{"smax": 8, **kw})):
+        for name in ("smax", "start"):
+            with pytest.raises(ValueError, match="2\\^31"):
+                call(**{name: big})
+    with pytest.raises(ValueError, match="2\\^31"):
+        calls[3](smax=big)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.kv4_cache(1, 2, big, 32, "cpu")
+    for size in (lambda w, p: ops.attn_window_fwd_workspace(1, 8, 8, 65536, 1, 64, window=w, prefix_len=p),
+                 lambda w, p: ops.attn_window_bwd_workspace(1, 8, 8, 65536, 1, 64, window=w, prefix_len=p),
+                 lambda w, p: ops.attn_window_decode_workspace(1, 8, 8, 64, 65536, window=w, prefix_len=p),
+                 lambda w, p: ops.attn_decode_kv4_workspace(1, 8, 8, 64, 65536, window=w, prefix_len=p)):
+        for w, p in ((big, 0), (0, big)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                size(w, p)
+
+
+def test_largest_numbers_that_fit_mean_no_limit():
+    top = (1 << 31) - 1
+    assert ops.attn_window_decode_workspace(2, 8, 2, 128, 65536, window=top) == ops.attn_window_decode_workspace(2, 8, 2, 128, 65536, window=0)
+    assert ops.attn_window_decode_workspace(2, 8, 2, 128, 65536, window=5, prefix_len=top) == ops.attn_window_decode_workspace(2, 8, 2, 128, 65536, window=0)
+
+
+def test_engine_refuses_a_window_past_32_bits():
+    from image_caption_amd.engine import DecoderEngine, EngineOptions, ModelGeometry
+    geo = ModelGeometry(64, 2, 128, 503)
+    DecoderEngine(geo, EngineOptions(mask_mode="window", window=(1 << 31) - 1))
+    for w in (1 << 31, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="window"):
+            DecoderEngine(geo, EngineOptions(mask_mode="window", window=w))
