@@ -102,6 +102,15 @@ extern "C" int capdec_decode_step_kv(const capdec_decode_desc* p, const capdec_d
     CAPDEC_CHECK((((uintptr_t)p->workspace) & (ALIGN - 1)) == 0, "decode_step: workspace must be 256-byte aligned");
     const StepBuffers s = carve((char*)p->workspace, B, d, ff, p->vocab, p->dtype, H, p->smax, kv);
     const int cdt = p->dtype;
+    // everything that a launch of step 2 could refuse, before step 1 has advanced ids, done and out
+    for (int i = 0; advance && i < p->n_blocks; ++i) {
+        const capdec_block_params& w = p->blocks[i];
+        CAPDEC_CHECK(w.kv_cache && w.in_proj_w && w.out_proj_w && w.linear1_w && w.linear2_w && w.norm1_w && w.norm1_b && w.norm2_w && w.norm2_b,
+                     "decode_step: block %d has a null weight", i);
+        CAPDEC_CHECK(!kv || !(kv->kv4 || kv->window > 0) || aligned16(w.kv_cache), "decode_step: block %d's cache must be 16-byte aligned", i);
+    }
+    CAPDEC_CHECK(!kv || !(kv->kv4 || kv->window > 0) || hd == 32 || hd == 64 || hd == 96 || hd == 128, "decode_step: head dim %d (32, 64, 96 or 128)", hd);
+    CAPDEC_CHECK(!kv || !(kv->kv4 || kv->window > 0) || p->smax < (1 << 28), "decode_step: smax %d", p->smax);
 
     // 1. score the newest row, pick the token, book-keep <eos>/<pad>
     // with the vocabulary matrix's image given, the newest rows are cast and laid out as an image in one pass
@@ -120,8 +129,6 @@ extern "C" int capdec_decode_step_kv(const capdec_decode_desc* p, const capdec_d
     const float scale = 1.0f / sqrtf((float)hd);
     for (int i = 0; i < p->n_blocks; ++i) {
         const capdec_block_params& w = p->blocks[i];
-        CAPDEC_CHECK(w.kv_cache && w.in_proj_w && w.out_proj_w && w.linear1_w && w.linear2_w && w.norm1_w && w.norm1_b && w.norm2_w && w.norm2_b,
-                     "decode_step: block %d has a null weight", i);
         CAPDEC_TRY(capdec_ln_fwd(xcur, w.norm1_w, w.norm1_b, p->ln_eps, B, d, s.hs, cdt, nullptr, nullptr, stream));
         capdec_gemm_desc g = linear(s.hs, w.in_proj_w, s.qs, B, 3 * d, d, cdt, cdt, w.in_proj_b);
         g.ldc = d;                                   // only the q columns reach C; K/V columns go to the cache

@@ -58,3 +58,38 @@ def test_engine_refuses_a_window_past_32_bits():
     for w in (1 << 31, (1 << 32) + 5):
         with pytest.raises(ValueError, match="window"):
             DecoderEngine(geo, EngineOptions(mask_mode="window", window=w))
+
+
+def decode_step(kv, **kw):
+    """The return code of a decoding step over made-up addresses, all of which the host must refuse (a launch would give -2 here)."""
+    import ctypes
+    from image_caption_amd import _lib
+    at = 1 << 20
+    nb = kw.pop("n_blocks", 2)
+    blocks = (_lib.BlockParams * nb)()
+    for i in range(nb):
+        for name, _ in _lib.BlockParams._fields_:
+            setattr(blocks[i], name, at)
+    for name, val in kw.pop("last", {}).items():
+        setattr(blocks[nb - 1], name, val)
+    d = _lib.DecodeDesc()
+    base = dict(B=2, d_model=64, nhead=2, dim_ff=128, vocab=100, n_blocks=nb, smax=40, dtype=_lib.BF16, ln_eps=1e-5, head_w=at, emb=at, x_last=at, ids=at,
+                done=at, out=at, max_len=8, t=0, s_new=20, workspace=at, workspace_bytes=1 << 40)
+    base.update(kw)
+    for name, val in base.items():
+        setattr(d, name, val)
+    d.blocks = blocks
+    lib = _lib.load()
+    return lib.capdec_decode_step_kv(ctypes.byref(d), kv, None), lib.capdec_last_error().decode()
+
+
+@pytest.mark.parametrize("four,window", [(1, 0), (0, 5), (1, 5)])
+def test_decode_step_refuses_before_it_advances_the_tokens(four, window):
+    from image_caption_amd import _lib
+    kv = _lib.DecodeKv(four, window, 3)
+    for bad, text in ((dict(d_model=96), "head dim 48"), (dict(last=dict(kv_cache=(1 << 20) + 8)), "aligned"), (dict(last=dict(kv_cache=None)), "null"),
+                      (dict(last=dict(linear2_w=None)), "null"), (dict(smax=1 << 28), "smax")):
+        rc, why = decode_step(kv, **bad)
+        assert rc == -1 and text in why, (bad, rc, why)
+    rc, why = decode_step(None, last=dict(norm2_b=None))
+    assert rc == -1 and "null" in why
