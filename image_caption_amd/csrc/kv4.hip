@@ -98,7 +98,7 @@ __device__ __forceinline__ unsigned k4_quantise(const float (&x)[32], unsigned c
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs p) {
     using G = K4<HD>;
-    __shared__ unsigned char lev[32][HD + 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lev[32][HD + 4];
     const int bh = blockIdx.x, b = bh / p.Hkv, h = bh - b * p.Hkv, tid = threadIdx.x;
     const long start = p.starts ? p.starts[b] : p.start;
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
