@@ -171,3 +171,37 @@ def test_one_kernel_backward_needs_no_workspace():
                 res.append(grads)
         if dtype == torch.bfloat16:
             assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*res))
+
+
+@pytest.mark.parametrize("dropout", [0.0, 0.1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mode,window,nb", [("prefix_window", 4, 2), ("window", 3, 1)])
+def test_model_gradients_repeat_bit_for_bit(mode, window, nb, dtype, dropout):
+    """The window kernels have no atomics, so every gradient that passes through them has the same bits each time; only linear1.bias, whose
+    column sums some of the framework's products form with atomics, and which feeds nothing else, may differ in its last ones."""
+    import helpers
+    from helpers import TINY
+    from oracle import ref_cpu
+    from image_caption_amd.engine import block_key
+    from test_parity_gpu import make_model
+    sds = [helpers.make_state_dict(TINY, seed=930 + i) for i in range(nb)]
+    full = dict(sds[0])
+    for i in range(1, nb):
+        for key in ref_cpu.BLOCK_KEYS:
+            full[block_key(i, key, nb)] = sds[i][key]
+    img, sos, cap, labels = (t.to(DEV) for t in helpers.make_embeddings(TINY, seed=609))
+    runs = []
+    for _ in range(3):
+        model = make_model(TINY, full, dtype, dropout=dropout, n_blocks=nb, mask_mode=mode, window=window, activation="gelu")
+        model.train()
+        loss, correct = model.caption_loss((img, sos, cap), labels)
+        loss.backward()
+        runs.append({"loss": loss.detach(), "correct": correct, **{key: p.grad for key, p in model.named_parameters()}})
+    for other in runs[1:]:
+        for key, t in runs[0].items():
+            assert torch.isfinite(t).all(), key
+            if key.endswith("linear1.bias"):
+                # sums of the same numbers in another order: a few units of the column's absolute sum, which 2^-16 of the largest covers
+                assert (t - other[key]).abs().max() <= 2.0 ** -16 * t.abs().max() + 1e-12, key
+            else:
+                assert torch.equal(t, other[key]), key
