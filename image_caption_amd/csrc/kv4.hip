@@ -465,7 +465,12 @@ int dec4_splits(int B, int H, int Hkv, int smax, int window, int prefix) {
     const int G = H / Hkv;
     const long wgs = (long)B * Hkv * ((G + 15) / 16);
     const long w = window == 0 || window > smax ? smax : window, seen = w + prefix < smax ? w + prefix : smax;
-    long ns = (1024 + wgs - 1) / wgs;                        // four workgroups per CU, none with fewer than four blocks for each wave
+    // Four workgroups per CU, none with fewer than four blocks for each wave.  Measured (us), not cut | aimed at 512 | 1024 | 2048
+    // workgroups, then 1024 of at least two | eight blocks a wave:
+    //   8 x 4096 rows, 32 heads on 8 of 128:  33 | 15.6 | 15.4 | 15.4,  17.1 | 15.7      1 x 4096: 32 | 10.7 | 10.7 | 10.7,  9.5 | 14.4
+    //   1 x 32768:                           234 | 18.2 | 17.9 | 17.7,  21.8 | 16.5      4 x 131072: 933 | 125 | 137 | 129,  136 | 136
+    //   32 x 1024, 8 heads of 96:            9.5 | 12.1 | 12.0 | 12.1,  12.3 | 9.4
+    long ns = (1024 + wgs - 1) / wgs;
     const long most = (seen / 32 + 2) / 16;
     if (ns > most) ns = most;
     if (ns > 1024) ns = 1024;

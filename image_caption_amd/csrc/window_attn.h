@@ -389,9 +389,16 @@ template <int HD> __device__ __forceinline__ void store_rows(const f32x16 (&acc)
 }
 
 // ------------------------------------------------------------------ host side
-// four waves on the keys of 32 rows instead of on 32 rows each: for few rows, and where tiles of 128 rows would leave CUs idle
-inline bool win_few_rows(long bh, long rows) { return rows <= 64 || bh * ((rows + 127) / 128) < 256; }
+// Four waves on the keys of 32 rows instead of on 32 rows each: for few rows, and where tiles of 128 rows would leave CUs idle.
+// Measured in us, waves on rows | on keys (hd 64, 229 keys unless said otherwise):
+//   forward, bf16, 2048 heads, 1 / 32 / 48 / 64 rows:  27.0 | 22.9   28.0 | 25.9   31.2 | 37.5   31.8 | 38.3     (hd 96: 39.8 | 40.0 at 32, 44.3 | 62.9 at 64)
+//   forward, f32, 2048 heads, 1 / 32 / 64 rows:        104 | 63      106 | 70      157 | 123
+//   backward, bf16, 2048 heads, 1 / 32 / 64 rows:      75.6 | 70.9   81.6 | 79.0   96.2 | 108.6                  (hd 128, where dQ spills: 179 | 196 at 32)
+//   backward, f32, 2048 heads, 1 / 32 / 64 rows:       410 | 371     421 | 398     570 | 593                     (hd 96: 640 | 467 at 32, 773 | 735 at 64)
+//   tiles of 128 rows on 16 CUs (2 x 8 heads of 229 rows, hd 96): 9.0 | 7.9, on 64 (1 head, 8192 rows, hd 128): 48.6 | 30.1,
+//   on 128: 9.3 | 10.2 and 19.8 | 16.4, on 256: 9.9 | 17.9 and 19.5 | 19.8
+inline bool win_few_rows(bool f32, long bh, long rows) { return rows <= (f32 ? 64 : 32) || bh * ((rows + 127) / 128) < 256; }
 int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what);
 struct WinFwdPlan { int kw; int tiles; int nsplit; long part_floats; };   // kw: four waves share the keys of 32 rows (else 4 x 32 rows)
-WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix);
+WinFwdPlan win_fwd_plan(bool f32, int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix);
 int win_fwd_launch(WinArgs& a, int dtype, int hd, void* workspace, long workspace_bytes, hipStream_t st);

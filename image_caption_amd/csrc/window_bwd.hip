@@ -767,7 +767,14 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
     long band = ((w + KT) * G + RB - 1) / RB;                              // and another one
     if (band > all) band = all;
     // enough workgroups for two per CU; a chunk's partial sums cost about what two steps do, so none has fewer than 16 steps
-    // -- unless the tiles do not even give every other CU a workgroup, where latency counts: two
+    // -- unless the tiles do not even give every other CU a workgroup, where latency counts: two.  Measured (us), not cut | aimed at
+    // 256 | 512 | 1024 workgroups, then 512 of at least 2 | 8 | 16 | 32 steps:
+    //   1 x 8192, 16 heads on 4 of 128, window 1024 + 4: 1780 | 333 | 309 | 332,  324 | 324 | 309 | 330
+    //   8 x 1024, 16 on 4 of 128, causal:                 266 | 266 | 227 | 213,  227 | 227 | 227 | 227
+    //   1 x 2048, 4 on 2 of 64, causal:                   158 |  56 |  52 |  61,   52 |  51 |  56 |  68
+    //   1 x 4100, 4 on 2 of 32, window 70 + 4:            407 |  37 |  36 |  36,   36 |  37 |  43 |  68
+    //   2 x 500, 8 on 2 of 128, causal:                   111 |  44 |  50 |  49,   49 |  47 |  61 | 113
+    //   3 x 333, 4 on 2 of 64, window 50, f32:             88 |  42 |  42 |  42,   42 |  88 |  88 |  88
     const long least = bh * pl.ktiles < 128 ? 2 : 16;
     auto chunks = [least](long wgs, long steps) {
         long c = wgs > 0 ? (512 + wgs - 1) / wgs : 1;
@@ -810,7 +817,7 @@ int bwd_go(WinArgs& a, hipStream_t st) {
         }
     }
     {
-        const bool kw = win_few_rows(bh, a.rows);
+        const bool kw = win_few_rows(sizeof(T) == 4, bh, a.rows);
         a.tiles = (a.rows + (kw ? 31 : 127)) / (kw ? 32 : 128);
         CAPDEC_CHECK(bh * a.tiles < (1L << 31), "attn_window_bwd: grid too large");
         auto go = [&](auto kfn, int lds) {

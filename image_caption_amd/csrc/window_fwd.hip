@@ -319,11 +319,11 @@ int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what) {
     return CAPDEC_OK;
 }
 
-WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix) {
+WinFwdPlan win_fwd_plan(bool f32, int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix) {
     WinFwdPlan pl;
     const int G = H / Hkv;
     const long rows = (long)nq * G;
-    pl.kw = win_few_rows((long)B * Hkv, rows);
+    pl.kw = win_few_rows(f32, (long)B * Hkv, rows);
     const int R = pl.kw ? 32 : 128, BK = pl.kw ? 128 : 64;
     pl.tiles = (int)((rows + R - 1) / R);
     // key tiles that a row tile can see at most
@@ -334,7 +334,11 @@ WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window
     const long nt = seen / BK + 2;
     const long wgs = (long)B * Hkv * pl.tiles;
     long ns = 1;
-    if (wgs < 512) {                     // two workgroups per CU, each with at least four key tiles of its own
+    // Two workgroups per CU, each with at least four key tiles of its own.  Measured (one token, us): not cut | as here | aimed at 1024
+    // workgroups | at least two tiles | eight:  8 x 1024 keys, hd 96: 13.5 | 12.5 | 12.6 | 10.1 | 13.5;  8 x 4096, hd 128: 50 | 13.8 | 13.8 | 11.7 | 19.5;
+    // 32 x 4096: 58 | 19.8 | 20.1 | 19.6 | 24.6;  8 x 32768: 428 | 31.0 | 30.9 | 31.0 | 30.4;  64 x 32768: 610 | 204 | 198 | 197 | 199;
+    // 8 x 131072: 2363 | 111 | 109 | 107 | 108.  (Two tiles would gain a third at small caches.)
+    if (wgs < 512) {
         ns = (512 + wgs - 1) / wgs;
         if (ns > nt / 4) ns = nt / 4;
         if (ns > 1024) ns = 1024;
@@ -346,7 +350,7 @@ WinFwdPlan win_fwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window
 }
 
 int win_fwd_launch(WinArgs& a, int dtype, int hd, void* workspace, long workspace_bytes, hipStream_t st) {
-    const WinFwdPlan pl = win_fwd_plan(a.B, a.H, a.Hkv, a.S, a.nq, hd, a.window >= (1 << 30) ? 0 : a.window, a.prefix);
+    const WinFwdPlan pl = win_fwd_plan(dtype == CAPDEC_F32, a.B, a.H, a.Hkv, a.S, a.nq, hd, a.window >= (1 << 30) ? 0 : a.window, a.prefix);
     a.tiles = pl.tiles;
     a.nsplit = 1;
     if (pl.nsplit > 1 && workspace) {
@@ -364,7 +368,9 @@ int win_fwd_launch(WinArgs& a, int dtype, int hd, void* workspace, long workspac
 
 extern "C" long capdec_attn_window_fwd_workspace(int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix_len) {
     if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || S <= 0 || nq <= 0 || hd <= 0 || window < 0 || prefix_len < 0) return 0;
-    return win_fwd_plan(B, H, Hkv, S, nq, hd, window, prefix_len).part_floats * 4;
+    // (either type's: the rows up to which the keys are shared out differ)
+    const long f32 = win_fwd_plan(true, B, H, Hkv, S, nq, hd, window, prefix_len).part_floats, bf16 = win_fwd_plan(false, B, H, Hkv, S, nq, hd, window, prefix_len).part_floats;
+    return (f32 > bf16 ? f32 : bf16) * 4;
 }
 
 extern "C" int capdec_attn_window_fwd(const capdec_attn_window_desc* d, void* stream) {

@@ -205,3 +205,30 @@ def test_model_gradients_repeat_bit_for_bit(mode, window, nb, dtype, dropout):
                 assert (t - other[key]).abs().max() <= 2.0 ** -16 * t.abs().max() + 1e-12, key
             else:
                 assert torch.equal(t, other[key]), key
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,H,Hkv,S,nq,hd,window,prefix", [
+    (40, 8, 8, 100, 48, 64, 20, 3),                                  # 33..64 rows and a tile for every CU: the waves split the rows in bf16, the keys in f32
+    (75, 8, 4, 900, 24, 32, 0, 0),                                   # the same with two heads to a K/V head, and few enough to cut along the keys
+    (35, 8, 8, 229, 33, 96, 16, 197),
+    (33, 8, 8, 300, 64, 128, 40, 0),
+    (70, 4, 4, 130, 32, 64, 0, 0),
+])
+def test_rows_between_the_two_shapes_of_workgroup(B, H, Hkv, S, nq, hd, window, prefix, dtype):
+    print(B, H, Hkv, S, nq, hd, window, prefix, dtype, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(23)
+    q, dout = (torch.randn(B, H, nq, hd, generator=g, device=DEV) * hd ** -0.5).to(dtype), torch.randn(B, H, nq, hd, generator=g, device=DEV).to(dtype)
+    k, v = (torch.randn(B, Hkv, S, hd, generator=g, device=DEV).to(dtype) for _ in range(2))
+    ns = [S - 17 * (b % 5) for b in range(B)]
+    lens = torch.tensor(ns, dtype=torch.int32, device=DEV)
+    kw = dict(window=window, prefix_len=prefix, q_start=S - nq)
+    see = wo.masks(B, S, nq, S - nq, ns, window, prefix, False, DEV)
+    want, want_lse, bound, _ = wo.forward(q, k, v, see)
+    o, lse, *grads = run(q, k, v, dout, lens=lens, **kw)
+    wo.assert_within(o, want, bound, "o")
+    whole = torch.full_like(q, float("nan"))
+    ops.attn_window_fwd(q, k, v, whole, lens=lens, **kw)
+    wo.assert_within(whole, want, bound, "o in one piece")
+    for got, (w, bd), what in zip(grads, wo.backward(q, k, v, o, lse, dout, see, 1.0), ("dq", "dk", "dv")):
+        wo.assert_within(got, w, bd, what)
