@@ -37,21 +37,33 @@ constexpr int RB = 32;               // rows per step
 // The common part c of the keys, for dQ: the mean of 64 keys from the middle of the longer run of visible ones, in the channels where it
 // stands out of the keys' own spread (five standard errors of that mean: what is below would only be the sample's noise, and an offset
 // of 0.6 spreads costs dQ less than the roundings do).  Fewer than 32 keys say nothing: c = 0.
-// Loads at the start of a workgroup, beside the first tile's; partial sums and squares meet in LDS.
+// Formed at the start of a workgroup; partial sums and squares meet in LDS.
 template <int HD, int NT> struct KeyMean {
-    static constexpr int N = 64, P = HD / 2, RG = NT / P, U = (N + RG - 1) / RG;      // channel pairs of a row, rows at a time, rows of a thread
+    static constexpr int N = 64, P = HD / 2, RG = NT >= 512 ? 8 : NT / P, U = (N + RG - 1) / RG;      // channel pairs of a row, rows at a time, rows of a thread
     static constexpr int PART = RG * HD * 8, BYTES = PART + HD * 4;
     unsigned x[U];
-    int m;
-    __device__ __forceinline__ void load(const bf16_t* k, long ss, const WinSpan& any, int tid) {
+    int key0, m;
+    __device__ __forceinline__ void pick(const WinSpan& any) {
         const bool one = any.lo <= any.a, band = !one && any.hi - any.lo >= any.a;
         const int first = band ? any.lo : 0, len = one ? max(any.a, any.hi) : band ? any.hi - any.lo : any.a;
         m = min(N, len);
-        const int key0 = first + (len - m) / 2, row = tid / P, pair = tid - row * P;
+        key0 = first + (len - m) / 2;
+    }
+    __device__ __forceinline__ void load(const bf16_t* k, long ss, int tid) {
+        const int row = tid / P, pair = tid - row * P;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             x[j] = 0;
             if (row < RG && row + j * RG < m) x[j] = *reinterpret_cast<const unsigned*>(k + (key0 + row + j * RG) * ss + 2 * pair);
+        }
+    }
+    // from K's rows in LDS (row 0 is key 0)
+    __device__ __forceinline__ void load(const char* lk, int tid) {
+        const int row = tid / P, pair = tid - row * P;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            x[j] = *reinterpret_cast<const unsigned*>(lk + WinGeo<bf16_t, HD>::at(max(0, key0 + min(row + j * RG, m - 1)), pair >> 2) + 4 * (pair & 3));
+            x[j] = row + j * RG < m ? x[j] : 0u;
         }
     }
     __device__ __forceinline__ void partial(char* lds, int tid) const {
@@ -151,7 +163,10 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
     };
     if (tl.nt > 0) {                   // (on its way before the rows are waited for)
         fetch(0);
-        if constexpr (CENTRE) mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, any, tid);
+        if constexpr (CENTRE) {
+            mean.pick(any);
+            mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, tid);
+        }
     }
     if (lse == -INFINITY) lse = INFINITY;              // a row that sees nothing: every probability is 0
     float delta = df.dot(of);
@@ -655,7 +670,6 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         }
         if (win_sees(any, key)) vf.load(reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hkv * p.v_hs + (long)key * p.v_ss, lane);
         fetch(0);
-        mean.load(reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hkv * p.k_hs, p.k_ss, any, tid);
 #pragma unroll
         for (int j = 0; j < NZ; ++j) {
             const int u = tid + 512 * j, row = u / CPR, c = u - row * CPR;
@@ -670,9 +684,10 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
 
     commit(0, smem);
-    mean.partial(lmean, tid);
     __syncthreads();
-    mean.finish(lmean, tid);                                                // (read after the first steps, each of which ends in a barrier)
+    mean.pick(any);
+    mean.load(lk, tid);                                                     // (read from memory once more: 2048 heads of 48 rows of 64 channels 97 -> 107 us)
+    mean.partial(lmean, tid);
     for (int blk0 = 0; blk0 < nblk; blk0 += 4) {
         for (int blk = blk0; blk < min(blk0 + 4, nblk); ++blk) {
             const bool more = blk + 1 < nblk;
@@ -689,6 +704,10 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
                     u32x2{win_pack(ds[4 * jj], ds[4 * jj + 1]), win_pack(ds[4 * jj + 2], ds[4 * jj + 3])};
             if (more) commit(blk + 1, smem + ((blk + 1) & 1) * L::BUF);
             __syncthreads();
+            if (blk == 0) {                                                 // (read after the next step's barrier)
+                mean.finish(lmean, tid);
+                if (!more) __syncthreads();
+            }
         }
         // 16x16x32 products: lane l holds column l & 15 of either operand and the keys 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3
         const int rb = wave & 3, half = wave >> 2;
