@@ -65,6 +65,12 @@ __device__ __forceinline__ WinSpan win_union(const WinArgs& p, int pos0, int pos
     s.a = live ? min(p.prefix, p.open ? n : s.hi) : 0;
     return s;
 }
+// How many of the first packed rows see one key alone: that key's probability is 1 whatever its score, so the score has no gradient,
+// which dP - delta, two sums of the same numbers in different orders, would only come near.  (A query past the first position
+// sees its own key and another one unless window 1 stands alone; an open prefix of two shows them to all.)
+__device__ __forceinline__ int win_single_rows(const WinArgs& p, int n) {
+    return p.window == 1 && p.prefix == 0 ? p.rows : p.q_start > 0 || (p.open && min(p.prefix, n) > 1) ? 0 : p.G;
+}
 // (bitwise, and used in selects only: a branch per element costs more, and a conditional store into a vector's element has
 // come out of the compiler without the store)
 __device__ __forceinline__ bool win_sees(const WinSpan& s, int key) { return (key < s.a) | ((key >= s.lo) & (key < s.hi)); }

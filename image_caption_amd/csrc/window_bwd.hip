@@ -259,13 +259,14 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
                 }
         }
     }
+    const float scale = !DROP && r < win_single_rows(p, n) ? 0.f : p.dq_scale;
     if constexpr (KW == 1) {
         T* out = reinterpret_cast<T*>(p.dq) + (long)b * p.dq_bs + (long)head * p.dq_hs + (long)irel * p.dq_ss;
-        store_rows<HD>(acc, p.dq_scale, out, r < p.rows, lane);
+        store_rows<HD>(acc, scale, out, r < p.rows, lane);
     } else {
         constexpr int PJ = HD + 4;
         float* jo = reinterpret_cast<float*>(smem);
-        store_rows<HD>(acc, p.dq_scale, jo + (kw * 32 + (lane & 31)) * PJ, true, lane);
+        store_rows<HD>(acc, scale, jo + (kw * 32 + (lane & 31)) * PJ, true, lane);
         __syncthreads();
         for (int u = tid; u < 32 * HD / 4; u += NT) {
             const int row = u / (HD / 4), c = (u - row * (HD / 4)) * 4, rr = r_first + row;
@@ -508,23 +509,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_dkv_kernel(Wi
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
 
+    const int single = DROP ? 0 : win_single_rows(p, n);          // (with dropout o is V scaled and rounded: delta is the formula's with that o)
     auto commit = [&](int blk, char* buf) {
         // rows of a block are in the order of their positions: those before the sequence's end come first
         // (queries are counted before they are multiplied by the heads: (S - q_start) * G may pass 32 bits, rows = nq * G does not)
         const int live = min(p.nq, max(0, n - p.q_start)) * p.G - blk * RB;
+        const int alone = single - blk * RB;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int u = tid + 256 * j, row = u / CPR, ch = u - row * CPR;
             if (RB * CPR % 256 == 0 || row < RB) {
                 const u32x4 z = {0, 0, 0, 0};
-                *reinterpret_cast<u32x4*>(buf + G::at(row, ch)) = row < live ? fq[j] : z;
+                *reinterpret_cast<u32x4*>(buf + G::at(row, ch)) = (row < live) & (row >= alone) ? fq[j] : z;
                 *reinterpret_cast<u32x4*>(buf + MAT + G::at(row, ch)) = row < live ? fd[j] : z;
             }
         }
         if (tid < RB) {
             float* st = reinterpret_cast<float*>(buf + 2 * MAT);
             // rows that are not there, and rows that see nothing: probability 0.  (bf16: in units of the exponent of 2)
-            st[tid] = tid >= live || f_lse == -INFINITY ? INFINITY : (sizeof(T) == 2 ? f_lse * WIN_LOG2E : f_lse);
+            // rows that see one key: probability 1 from a score of 0, and nothing for dK
+            st[tid] = tid >= live || f_lse == -INFINITY ? INFINITY : tid < alone ? 0.f : (sizeof(T) == 2 ? f_lse * WIN_LOG2E : f_lse);
             st[RB + tid] = tid >= live ? 0.f : f_delta;
             reinterpret_cast<int*>(st)[2 * RB + tid] = p.q_start + win_row_query(p, min(blk * RB + tid, p.rows - 1));
         }
@@ -628,6 +632,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
     const int che = (loads ? ch : 0) * 8;
     u32x4 fq, fd, fo;
     float f_lse;
+    const int single = DROP ? 0 : win_single_rows(p, n);
     auto fetch = [&](int blk) {
         const int r = min(blk * RB + srow, p.rows - 1), i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
         fq = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i * p.q_ss + che);
@@ -637,11 +642,12 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
     };
     auto commit = [&](int blk, char* buf) {
         const bool live = srow < min(p.nq, max(0, n - p.q_start)) * p.G - blk * RB;
+        const bool alone = srow < single - blk * RB;
         const u32x4 z = {0, 0, 0, 0};
         fd = live ? fd : z;
         fo = live ? fo : z;
         if (loads) {
-            *reinterpret_cast<u32x4*>(buf + G::at(srow, ch)) = live ? fq : z;
+            *reinterpret_cast<u32x4*>(buf + G::at(srow, ch)) = live & !alone ? fq : z;
             *reinterpret_cast<u32x4*>(buf + L::MAT + G::at(srow, ch)) = fd;
         }
         const bf16x8 x = __builtin_bit_cast(bf16x8, fd), y = __builtin_bit_cast(bf16x8, fo);
@@ -651,7 +657,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
         delta = sum16(loads ? delta : 0.f);
         if (ch == 0) {
             float* st = reinterpret_cast<float*>(buf + 2 * L::MAT);
-            st[srow] = !live || f_lse == -INFINITY ? INFINITY : f_lse * WIN_LOG2E;
+            st[srow] = !live || f_lse == -INFINITY ? INFINITY : alone ? 0.f : f_lse * WIN_LOG2E;
             st[RB + srow] = delta;
             reinterpret_cast<int*>(st)[2 * RB + srow] = p.q_start + win_row_query(p, min(blk * RB + srow, p.rows - 1));
         }
@@ -758,10 +764,11 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
                 if (r >= p.rows) continue;
                 const int i = win_row_query(p, r), h = hkv * p.G + r - i * p.G;
                 T* out = reinterpret_cast<T*>(p.dq) + (long)b * p.dq_bs + (long)h * p.dq_hs + (long)i * p.dq_ss + half * (HD / 2) + 4 * g;
+                const float scale = r < single ? 0.f : p.dq_scale;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-                    *reinterpret_cast<u32x2*>(out + 16 * t) = u32x2{win_pack(acc[rh][t][0] * p.dq_scale, acc[rh][t][1] * p.dq_scale),
-                                                                    win_pack(acc[rh][t][2] * p.dq_scale, acc[rh][t][3] * p.dq_scale)};
+                    *reinterpret_cast<u32x2*>(out + 16 * t) = u32x2{win_pack(acc[rh][t][0] * scale, acc[rh][t][1] * scale),
+                                                                    win_pack(acc[rh][t][2] * scale, acc[rh][t][3] * scale)};
             }
         }
         if (blk0 + 4 < nblk) __syncthreads();                               // the next step writes dS where this one was read

@@ -232,3 +232,42 @@ def test_rows_between_the_two_shapes_of_workgroup(B, H, Hkv, S, nq, hd, window, 
     wo.assert_within(whole, want, bound, "o in one piece")
     for got, (w, bd), what in zip(grads, wo.backward(q, k, v, o, lse, dout, see, 1.0), ("dq", "dk", "dv")):
         wo.assert_within(got, w, bd, what)
+
+
+# B, H, Hkv, S, nq, hd, window, prefix, open, lens: a sequence of one, window 1 alone, a first row that sees itself, prefixes that add a key or do not
+ALONE = [
+    (3, 8, 2, 1, 1, 32, 1, 1, True, None),
+    (2, 2, 2, 1, 1, 64, 0, 0, False, None),
+    (300, 1, 1, 1, 1, 96, 0, 4, True, None),
+    (2, 8, 4, 200, 200, 64, 1, 0, False, None),
+    (2, 8, 4, 300, 300, 128, 1, 0, False, (300, 131)),
+    (40, 8, 8, 140, 50, 64, 1, 0, True, None),
+    (2, 4, 2, 300, 300, 32, 20, 3, False, None),
+    (2, 4, 4, 90, 90, 96, 5, 1, True, None),
+    (2, 4, 4, 90, 90, 128, 1, 1, True, None),
+    (3, 4, 4, 150, 150, 64, 30, 5, True, (150, 1, 2)),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", ALONE)
+def test_a_query_that_sees_one_key_has_no_gradient_for_its_score(case, dtype):
+    """Its probability is 1 whatever the score: its dQ and its share of dK are 0, not what two sums of the same numbers leave."""
+    B, H, Hkv, S, nq, hd, window, prefix, is_open, spec = case
+    print(case, dtype, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(29)
+    q, dout = (torch.randn(B, H, nq, hd, generator=g, device=DEV) * hd ** -0.5).to(dtype), torch.randn(B, H, nq, hd, generator=g, device=DEV).to(dtype)
+    k, v = (torch.randn(B, Hkv, S, hd, generator=g, device=DEV).to(dtype) for _ in range(2))
+    ns = [S] * B if spec is None else list(spec)
+    lens = None if spec is None else torch.tensor(ns, dtype=torch.int32, device=DEV)
+    kw = dict(window=window, prefix_len=prefix, prefix_open=is_open, q_start=S - nq)
+    see = wo.masks(B, S, nq, S - nq, ns, window, prefix, is_open, DEV)
+    alone = see.sum(-1) == 1                                              # [B, nq]
+    assert alone.any()
+    o, lse, dq, dk, dv = run(q, k, v, dout, lens=lens, **kw)
+    assert not dq[alone[:, None].expand(B, H, nq)].any()
+    others = (see & ~alone[:, :, None]).any(1)                            # [B, S]: keys that some other query sees
+    assert not dk[~others[:, None].expand(B, Hkv, S)].any()
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+    for got, (want, bound), what in zip((dq, dk, dv), wo.backward(q, k, v, o, lse, dout, see, 1.0), ("dq", "dk", "dv")):
+        wo.assert_within(got, want, bound, what)
