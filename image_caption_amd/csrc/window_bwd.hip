@@ -16,11 +16,12 @@
 // and what the keys have in common is multiplied by that sum: with channel offsets of 2 and 8 times the keys' spread dQ was
 // 0.009 and 0.035 of its size off.  In exact numbers the sum is 0 and any c may be taken out of the keys, so
 //     dQ = sum_j dS_j K_j - (sum_j dS_j) c,     the sum over the rounded dS, c the common part of some of the visible keys
-// (KeyMean below): one number a row, a 2-term dot product per two elements of dS.  dQ then lies 0.0024-0.0030 of its size from the exact one
-// whatever the offset, dK 0.0024-0.0025, against 0.0017 for their own rounding alone (cost: captioning stack 123.0 -> 127.6 us, 3 of them the
-// dot products, long case 318 -> 321; the sums by matrix instructions against ones 128.3).  With an exact delta -- S and dP a second time,
-// two products of seven -- it would be 0.0023-0.0026, which no half step of the output asks for.  What V's rows have in common
-// reaches delta through o's rounding and stays: an offset of twice V's spread, and dQ and dK lie at 0.005, eight times, at 0.02.
+// (KeyMean below): one number a row, a 2-term dot product per two elements of dS.  dQ then lies 0.0024-0.0035 of its size from the exact one
+// whatever the offset, dK 0.0024-0.0025, dV 0.0023, against 0.0017 for their own rounding alone.  Cost: captioning stack 123.0 -> 127.6 us, 3 of
+// them the dot products (sums by matrix instructions against ones: 128.3), 8192 positions 318 -> 321, 100 rows over 10000 keys 98 -> 109.
+// What V's rows have in common reaches delta through o's rounding, stays in the formula and is left: 0.005 of dQ and dK for an offset of
+// twice V's spread, 0.02 for eight times, and 0.005 of dQ where 9000 keys are averaged over an offset of a quarter.  An exact delta, 0.0023-0.0026,
+// would take S and dP a second time, two products of seven.
 //
 // Measured (bf16, us): 8192 positions, 16 heads on 4 of 128 channels, window 1024: dQ 122, dK / dV 190, join 19, 305-315 in all = 530 TFLOP/s
 // of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time: a step is one chain of
@@ -34,46 +35,53 @@ namespace {
 constexpr int KT = 128;              // keys of a dK / dV workgroup: four waves of 32
 constexpr int RB = 32;               // rows per step
 
-// The common part c of the keys, for dQ: the mean of 64 keys from the middle of the longer run of visible ones, in the channels where it
-// stands out of the keys' own spread (five standard errors of that mean: what is below would only be the sample's noise, and an offset
-// of 0.6 spreads costs dQ less than the roundings do).  Fewer than 32 keys say nothing: c = 0.
-// Formed at the start of a workgroup; partial sums and squares meet in LDS.
+// The common part c of the keys, for dQ: the mean of m keys spread over the longer run of visible ones, in the channels where it stands out
+// of the keys' own spread (five standard errors of that mean: what is below would only be the sample's noise).  One key in sixteen,
+// 64 at least and 1024 at most: what is left of c costs dQ less than its roundings do with 64 keys up to about a thousand,
+// and dQ, a mean over n keys, shrinks like 1 / sqrt(n) against it (100 rows over 10000 keys, 0.0074 of dQ with 64).  Fewer than 32
+// keys say nothing: c = 0.  Formed at the start of a workgroup; partial sums and squares meet in LDS.
 template <int HD, int NT> struct KeyMean {
-    static constexpr int N = 64, P = HD / 2, RG = NT >= 512 ? 8 : NT / P, U = (N + RG - 1) / RG;      // channel pairs of a row, rows at a time, rows of a thread
+    static constexpr int N = 64, P = HD / 2, RG = NT >= 512 ? 8 : NT / P, U = (N + RG - 1) / RG;      // channel pairs of a row, rows at a time, rows of a thread in N
     static constexpr int PART = RG * HD * 8, BYTES = PART + HD * 4;
     unsigned x[U];
-    int key0, m;
+    int key0, step, m;
+    f32x4 s;                                                                 // sum and squares of either channel
     __device__ __forceinline__ void pick(const WinSpan& any) {
         const bool one = any.lo <= any.a, band = !one && any.hi - any.lo >= any.a;
         const int first = band ? any.lo : 0, len = one ? max(any.a, any.hi) : band ? any.hi - any.lo : any.a;
-        m = min(N, len);
-        key0 = first + (len - m) / 2;
+        m = min(len, max(N, min(1024, len >> 4)));
+        step = m > 0 ? len / m : 1;
+        key0 = first + (len - 1 - (m - 1) * step) / 2;
+        s = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ void load(const bf16_t* k, long ss, int tid) {
+    // keys base.. of the sample
+    __device__ __forceinline__ void load(const bf16_t* k, long ss, int base, int tid) {
         const int row = tid / P, pair = tid - row * P;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
+            const int i = base + row + j * RG;
             x[j] = 0;
-            if (row < RG && row + j * RG < m) x[j] = *reinterpret_cast<const unsigned*>(k + (key0 + row + j * RG) * ss + 2 * pair);
+            if (row + j * RG < N && row < RG && i < m) x[j] = *reinterpret_cast<const unsigned*>(k + (long)(key0 + i * step) * ss + 2 * pair);
         }
     }
-    // from K's rows in LDS (row 0 is key 0)
+    // from K's rows in LDS (row 0 is key 0), of at most N keys
     __device__ __forceinline__ void load(const char* lk, int tid) {
         const int row = tid / P, pair = tid - row * P;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            x[j] = *reinterpret_cast<const unsigned*>(lk + WinGeo<bf16_t, HD>::at(max(0, key0 + min(row + j * RG, m - 1)), pair >> 2) + 4 * (pair & 3));
+            x[j] = *reinterpret_cast<const unsigned*>(lk + WinGeo<bf16_t, HD>::at(max(0, key0 + min(row + j * RG, m - 1) * step), pair >> 2) + 4 * (pair & 3));
             x[j] = row + j * RG < m ? x[j] : 0u;
         }
     }
-    __device__ __forceinline__ void partial(char* lds, int tid) const {
-        const int row = tid / P, pair = tid - row * P;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};                                      // sum and squares of either channel
+    __device__ __forceinline__ void add() {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const float lo = __uint_as_float(x[j] << 16), hi = __uint_as_float(x[j] & 0xFFFF0000u);
             s = f32x4{s[0] + lo, fmaf(lo, lo, s[1]), s[2] + hi, fmaf(hi, hi, s[3])};
         }
+    }
+    __device__ __forceinline__ void partial(char* lds, int tid) const {
+        const int row = tid / P, pair = tid - row * P;
         if (row < RG) *reinterpret_cast<f32x4*>(lds + (row * HD + 2 * pair) * 8) = s;
     }
     // (after a barrier; c may be read after another one)
@@ -165,7 +173,7 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
         fetch(0);
         if constexpr (CENTRE) {
             mean.pick(any);
-            mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, tid);
+            mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, 0, tid);
         }
     }
     if (lse == -INFINITY) lse = INFINITY;              // a row that sees nothing: every probability is 0
@@ -218,10 +226,20 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
             else mma_cols<HD>(acc, lk, s, at);
         }
     };
+    auto sample = [&] {
+        if constexpr (CENTRE) {
+            mean.add();
+            for (int base = mean.N; base < mean.m; base += mean.N) {
+                mean.load(reinterpret_cast<const T*>(kbase), p.k_ss, base, tid);
+                mean.add();
+            }
+            mean.partial(lmean, tid);
+        }
+    };
     if (tl.nt > 0) {
         if constexpr (NBUF == 2) {
             commit(0, smem, smem + MAT);
-            if constexpr (CENTRE) mean.partial(lmean, tid);
+            sample();
             __syncthreads();
             if constexpr (CENTRE) mean.finish(lmean, tid);
             for (int idx = 0; idx < tl.nt; ++idx) {
@@ -233,8 +251,8 @@ __global__ __launch_bounds__(64 * QW * KW, sizeof(T) == 2 ? 2 : 1) void win_dq_k
                 __syncthreads();
             }
         } else {
+            sample();
             if constexpr (CENTRE) {
-                mean.partial(lmean, tid);
                 __syncthreads();
                 mean.finish(lmean, tid);
             }
@@ -693,6 +711,7 @@ __global__ __launch_bounds__(512, 2) void win_bwd_short_kernel(WinArgs p) {
     __syncthreads();
     mean.pick(any);
     mean.load(lk, tid);                                                     // (read from memory once more: 2048 heads of 48 rows of 64 channels 97 -> 107 us)
+    mean.add();
     mean.partial(lmean, tid);
     for (int blk0 = 0; blk0 < nblk; blk0 += 4) {
         for (int blk = blk0; blk < min(blk0 + 4, nblk); ++blk) {
