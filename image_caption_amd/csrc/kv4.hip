@@ -1,7 +1,8 @@
 // A K/V cache held in 4 bits per value, and attention of one token per sequence over it.
 //
 // Format.  A row (one position, one head, K or V) is cut into groups of 32 channels; a group keeps a bf16 scale and a bf16
-// offset next to its 32 levels 0..15, and stands for offset + scale * level (exact in f32):
+// offset next to its 32 levels 0..15, and stands for offset + scale * level (scale * level is exact in f32, the sum is rounded
+// once on read-back; the attention applies offset and scale apart, so it can differ from that in the last bit):
 //     offset = bf16(min), scale = bf16((max - min) * f32(1/15)), level = clamp(rint((x - offset) * (1 / scale)), 0, 15)
 // in f32 steps (all levels 0 where the scale is 0).  5 bits a value against 16.
 //
@@ -24,12 +25,12 @@
 // In f32 the levels become n - 7.5 instead (more instructions; 1 + n/16 costs the sums 23.5 / 4.6 of their digits), q and
 // p scale_t are split into three bf16 parts, which together are the f32 numbers: three products instead of one, on matrix
 // cores that are idle most of the time anyway.
-// What bounds it is HBM: 5 bits a value, read once.  Four waves of a workgroup take alternate blocks of 32 keys, each with its next block's
+// What bounds it is HBM: 5 bits a value, read once (the vector unit is active 0.52-0.62 of the time, unpacking).  Four waves of a workgroup take alternate blocks of 32 keys, each with its next block's
 // loads in flight, and join at the end; few sequences are cut along the keys, joined by kv4_join_kernel.
 //
-// Measured (bf16, us): 4 sequences of up to 131072 rows (32 heads on 8 of 128) 85 = 410 MB at 4.8 TB/s, the vector unit busy for half of it; 256
-// sequences of 229 rows (8 heads of 96) 16 = 57 MB at 3.6 TB/s, two blocks a wave, the rest is starting and joining.  Append of
-// 256 x 198 rows 49 (4.2 TB/s read and written), read-back of them to f32 66 (5.4 TB/s).
+// Measured (bf16, us): 4 sequences of up to 131072 rows (32 heads on 8 of 128) 85 = 410 MB at 4.8 TB/s; 256
+// sequences of 229 rows (8 heads of 96) 14.4-16 = 57 MB at 3.6-4 TB/s, two blocks a wave, the rest is starting and joining.  Append of
+// 256 x 198 rows 65 (3.2 TB/s read and written; 48 when nothing wrote before it), read-back of them to f32 70 (5.1 TB/s).
 #include "common.h"
 
 namespace {

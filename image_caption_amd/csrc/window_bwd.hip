@@ -23,8 +23,8 @@
 // twice V's spread, 0.02 for eight times, and 0.005 of dQ where 9000 keys are averaged over an offset of a quarter.  An exact delta, 0.0023-0.0026,
 // would take S and dP a second time, two products of seven.
 //
-// Measured (bf16, us): 8192 positions, 16 heads on 4 of 128 channels, window 1024: dQ 122, dK / dV 190, join 19, 305-315 in all = 530 TFLOP/s
-// of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time: a step is one chain of
+// Measured (bf16, us): 8192 positions, 16 heads on 4 of 128 channels, window 1024: dQ 127, dK / dV 190, join 19, 313-327 in all = 500-520 TFLOP/s
+// of the five products the formulas have (seven are made).  The matrix cores are busy a third of the time (0.35, 0.31): a step is one chain of
 // LDS reads, products, exponentials, products, LDS writes and a barrier, and only two waves a SIMD are there to fill it (the
 // accumulators of 64 + 64 registers and V's rows allow no third).  Left out in turn: dK and dV's products -52, LDS writes
 // -37, S and dP's products -32, loads from L2 -9, exponentials -5.  Two key blocks a wave at one wave a SIMD: 425.
@@ -614,8 +614,8 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinArgs p) {
 // (bf16, as both products take it) also goes to LDS as [key][row], and after every four steps each wave multiplies half of the
 // channels of one of the four blocks' dQ out of it: dQ^T = K^T dS^T with both operands read by columns.  Five products instead of
 // seven, q, k, v and dO read once instead of twice, and delta formed where dO passes by.  1024 heads of 229 rows of 96 channels:
-// 130 us against 159 for the two kernels; the 360 MB alone take 77, the rest is the phases of a CU's one workgroup (140 KB of
-// LDS, eight waves of 220 registers) following each other: K and V 26, the last stores 21, dQ 20.  One workgroup per CU that
+// 126-130 us against 147 for the two kernels; the 360 MB alone take 77, the rest is the phases of a CU's one workgroup (147 KB of
+// LDS, eight waves of 217 registers) following each other: K and V 26, the last stores 21, dQ 20.  One workgroup per CU that
 // loads its next head's K and V during dQ measured the same, and so did dQ's reads a block ahead.
 constexpr int SK = 256;
 template <int HD> struct ShortGeo {
@@ -836,10 +836,11 @@ BwdPlan bwd_plan(int B, int H, int Hkv, int S, int nq, int hd, int window, int p
 
 // One kernel for short sequences in bf16: where its workgroups, one per K/V head, fill the card or have few rows to go over one
 // after the other.  Measured in us, one kernel against the two (229 keys, all rows | 32 rows; H = Hkv):
-//   96 channels,  16 heads:  26 /  26 |  8 / 14     64 channels,  16 heads:  23 / 23      32 channels,  16 heads: 23 / 17
-//                256 heads:  34 /  44 | 14 / 21                  256 heads:  29 / 37                   256 heads: 26 / 28
-//                512 heads:  65 /  82 | 27 / 35                  512 heads:  54 / 67                   512 heads: 48 / 40
-// (and 64 keys, 512 heads: 19 / 27, 15 / 23, 15 / 15).  With 32 channels the products are too small a part of a step; with 128 the
+//   96 channels,  16 heads:  26 /  26 |  9 / 15     64 channels,  16 heads:  24 /  23 |  8 / 14     32 channels,  16 heads: 23 / 17 |  7 / 11
+//                256 heads:  35 /  43 | 14 / 21                  256 heads:  31 /  37 | 11 / 18                  256 heads: 27 / 29 |  8 / 13
+//                512 heads:  62 /  79 | 27 / 35                  512 heads:  56 /  63 | 22 / 27                  512 heads: 51 / 42 | 15 / 18
+//               1024 heads: 126 / 147                           1024 heads: 105 / 102                           1024 heads: 96 / 72
+// (and 64 keys, 512 heads: 19 / 21, 16 / 17, 16 / 14).  With 32 channels the products are too small a part of a step; with 128 the
 // accumulators, V and the fragments no longer fit the registers.
 template <typename T, int HD> constexpr bool HAS_SHORT = sizeof(T) == 2 && (HD == 64 || HD == 96);
 bool win_bwd_short(long bh, long rows, int S) { return S <= SK && (rows <= 256 || bh >= 256); }

@@ -14,11 +14,11 @@
 // Where the row tiles alone do not fill the GPU, the visible tiles of a row tile are cut into nsplit parts that leave
 // (O, m, l) in the workspace, joined by win_join_kernel.
 //
-// Measured (bf16, us): the scored rows of a captioning batch of 256 (32 of 229 rows, 8 heads of 96) 41 = 205 MB at 5.0 TB/s; one token of
-// 32 sequences of up to 32768 rows (32 heads on 8, 128 channels, window 8192) 198 = 1.08 GB at 5.5 TB/s: HBM bounds both.  A
-// prompt of 2 x 8192 (32 heads on 8, 128 channels, window 1024) 336 = 770 TFLOP/s: the matrix cores are busy 40 % of it, the vector
-// unit (32 exponentials a lane and tile above all) about as long, one wave's products only partly under the other's
-// exponentials.  Left out in turn: exp -26, reads of V -25, of K -50, global loads -40, their way to LDS -20.  Three waves a SIMD,
+// Measured (bf16, us): the scored rows of a captioning batch of 256 (32 of 229 rows, 8 heads of 96) 42 = 205 MB at 4.9 TB/s (49 a call); one token of
+// 32 sequences of up to 32768 rows (32 heads on 8, 128 channels, window 8192) 197 = 1.08 GB at 5.5 TB/s: HBM bounds both.  A
+// prompt of 2 x 8192 (32 heads on 8, 128 channels, window 1024) 334 = 770 TFLOP/s: the matrix cores are busy 37 % of it, the vector
+// unit (32 exponentials a lane and tile above all) 41 %, one wave's products only partly under the other's
+// exponentials; a tenth of both falls on keys that no row of the wave sees, a tile being left out only as a whole.  Left out in turn: exp -26, reads of V -25, of K -50, global loads -40, their way to LDS -20.  Three waves a SIMD,
 // one key half at a time, and the next tile's scores before this one's products measured the same.
 #include "window_attn.h"
 

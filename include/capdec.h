@@ -294,7 +294,8 @@ int capdec_attn_window_decode(const void* q, const void* kv_cache, void* o, int 
 /* ------------------------------------------------------------------ K/V cache in 4 bits per value
  * No reference counterpart.  A row of hd channels is cut into groups of 32; a group stands for offset + scale * level with
  * levels 0..15 and, in f32 steps, offset = bf16(min), scale = bf16((max - min) * f32(1/15)), level = clamp(rint((x - offset) *
- * (1 / scale)), 0, 15) (0 where the scale is 0).  A group that holds a NaN or an infinity stands for unspecified values.
+ * (1 / scale)), 0, 15) (0 where the scale is 0).  A group that holds a NaN or an infinity, or whose span passes f32's range or lies below 2^-126,
+ * stands for unspecified values.
  * The layout is the library's own: one piece of capdec_kv4_head_bytes(smax, hd) bytes per (sequence, K/V head), [B][Hkv]
  * pieces, 16-byte aligned; hd 32, 64, 96 or 128, smax < 2^28. */
 long capdec_kv4_head_bytes(int smax, int hd);
@@ -307,7 +308,7 @@ typedef struct {
     int dtype, n;
 } capdec_kv4_rows;
 
-/* Quantises n new rows of every sequence into rows start.. of the cache.  starts [B] int32 on the device (NULL: `start` for all): where each sequence's rows go; rows that would fall outside
+/* Quantises n new rows of every sequence (at most 2^21 - 64 a call) into rows start.. of the cache.  starts [B] int32 on the device (NULL: `start` for all): where each sequence's rows go; rows that would fall outside
  * 0..smax-1 are dropped.  counts [B] int32 on the device (NULL: n for all): how many of the n rows each sequence has, taken
  * into 0..n.  Other rows of the cache keep what they hold.  Two calls that may overlap in time must not write the same
  * 32-row block of a sequence. */
