@@ -8,8 +8,8 @@ on one synthetic Flickr-shaped batch that is already resident in HBM: prefix joi
 (img_text_concat.py:115-123) -> TransformerDecoder forward (dropout 0.1 active) ->
 cross-entropy over the 32 caption rows + argmax count -> backward -> Adam with
 coupled weight decay -> (N > 1) RCCL gradient all-reduce.  Workload at N=1:
-BASELINE.json configs[1] (batch 256, bf16, config.py defaults); each extra GPU adds
-another 256 samples (weak scaling; N=8 is configs[2]'s global batch 2048).
+batch 256, bf16, config.py defaults; each extra GPU adds
+another 256 samples (weak scaling; at N=8 the global batch is 2048).
 For N > 1 launch with torch.distributed.run, one rank per GPU.
 
 Rank 0 prints ONE JSON line.  Besides the contract fields it carries
@@ -17,11 +17,11 @@ Rank 0 prints ONE JSON line.  Besides the contract fields it carries
                 timed region, against the dense bf16 MFMA peak
   cpu_baseline  the reference's step as written (stock torch.nn, f32, CPU; oracle/),
                 timed on this host's cores at the reference's batch size 8 (and once at 64)
-  global_2048   configs[2] at THIS N: the same step at a fixed global batch of 2048
+  global_2048   at THIS N: the same step at a fixed global batch of 2048
                 (2048 / N samples per GPU), so a 1/2/4/8 sweep also yields the strong-scaling curve
-  greedy        KV-cached greedy captioning of 4096 images (configs[3]), N=1 only, with the
+  greedy        KV-cached greedy captioning of 4096 images, N=1 only, with the
                 full-recompute loop around the CPU oracle timed beside it
-  scaled        configs[4] (12 blocks, 257 patches, prefix-causal mask), N=1 only
+  scaled        12 blocks, 257 patches, prefix-causal mask, N=1 only
 """
 import argparse
 import json
@@ -429,7 +429,7 @@ def main():
     loss = out[0].item() / out[2]
     slab = model.engine.last_slab
 
-    # configs[2] at this N: the same step at a fixed global batch of 2048 (every rank takes part: same collectives)
+    # at this N: the same step at a fixed global batch of 2048 (every rank takes part: same collectives)
     g2048 = None
     if not args.no_global_2048 and not args.global_batch and args.n_blocks == 1 and 2048 % world == 0:
         Bg = 2048 // world
@@ -494,7 +494,7 @@ def main():
 
 
 def scaled_bench(build, timed, args):
-    """configs[4]: 12 blocks, 257 patches (S = 290), prefix-causal mask, 50260-token vocabulary, batch 256, one GPU."""
+    """12 blocks, 257 patches (S = 290), prefix-causal mask, 50260-token vocabulary, batch 256, one GPU."""
     B, P, nb = 256, 257, 12
     model, trainer = build(nb, "prefix_causal", args.activation)
     elapsed, out, _ = timed(model, trainer, B, P, 10, 3, 20, spans_wanted=False)
@@ -518,7 +518,7 @@ def scaled_bench(build, timed, args):
 
 
 def greedy_bench(model, dev, args):
-    """configs[3]: KV-cached greedy captioning of 4096 synthetic images, L=32, one GPU."""
+    """KV-cached greedy captioning of 4096 synthetic images, L=32, one GPU."""
     from image_caption_amd.synthetic import make_batch
     n = args.greedy_images
     model.eval()

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Attention forward / backward timings at the two training shapes: scored rows of the one-block model
-(S = 229, last 32 queries) and all rows of the stacked model (S = 290).  Usage (GPU box): python tools/attn_bench.py"""
+(S = 229, last 32 queries) and all rows of the stacked model (S = 290).  Usage (on an MI355X): python tools/attn_bench.py"""
 import os
 import sys
 

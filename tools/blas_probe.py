@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """What the vendor library (torch.matmul -> hipBLASLt) reaches on the vocabulary-stage products, as a yardstick for
 the hand-written kernels.  Diagnostic only: nothing in the package calls torch.matmul.
-Usage (on the GPU box): python tools/blas_probe.py"""
+Usage (on an MI355X): python tools/blas_probe.py"""
 import torch
 
 DEV, BF = "cuda", torch.bfloat16

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """A/B of the kernels that can run the fused logits + cross-entropy forward at the benchmark's size
 (8192 x 50260 x 768), interleaved in one process; each variant is also checked against the default one.
-Usage (on the GPU box): python tools/ce_fwd_ab.py [modes...]"""
+Usage (on an MI355X): python tools/ce_fwd_ab.py [modes...]"""
 import ctypes
 import os
 import sys

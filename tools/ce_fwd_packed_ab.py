@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """A/B of the persistent logits + cross-entropy forward with its operands read row-major against the same launch
 reading k-panel images ([K/32][rows][32]) of them, at the benchmark's size (8192 x 50260 x 768); results compared.
-Usage (on the GPU box): python tools/ce_fwd_packed_ab.py"""
+Usage (on an MI355X): python tools/ce_fwd_packed_ab.py"""
 import ctypes
 import os
 import sys

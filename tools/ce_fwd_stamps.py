@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Clock stamps of the logits + cross-entropy forward under a forced kernel geometry.
-Usage (on the GPU box): python tools/ce_fwd_stamps.py [modes...]"""
+Usage (on an MI355X): python tools/ce_fwd_stamps.py [modes...]"""
 import ctypes
 import os
 import sys

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Repeats the persistent logits + cross-entropy forward under disturbed cache / timing conditions and checks every
 launch bit for bit against its own first result, and that one against the generic kernel.
-Usage (on the GPU box): python tools/ce_fwd_stress.py [mode] [reps]"""
+Usage (on an MI355X): python tools/ce_fwd_stress.py [mode] [reps]"""
 import ctypes
 import os
 import sys

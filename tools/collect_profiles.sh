@@ -1,9 +1,9 @@
 #!/bin/bash
-# Collects the committed profile set on the GPU box, in steady state: every rocprofv3 pass runs bench.py with its default
+# Collects the committed profile set on an MI355X, in steady state: every rocprofv3 pass runs bench.py with its default
 # spin-up (150 untimed steps) and without the trailing stage-bracket steps, so the trace ends with the timed steps.
 #   bench line; rocprofv3 kernel stats (whole run) + statistics of the TIMED steps only + timeline of a timed step;
 #   HBM-side traffic (FETCH_SIZE / WRITE_SIZE, separate passes); MFMA utilisation; the same for the 12-block leg.
-# Results land in gpurun_out/.   Usage (through gpurun): bash tools/collect_profiles.sh [tag, default r03]
+# Results land in gpurun_out/.   Usage: bash tools/collect_profiles.sh [tag, default r03]
 set -e
 V=${1:-r03}
 cd /tmp && export TMPDIR=/tmp

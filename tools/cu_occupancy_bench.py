@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """How the vocabulary-stage and block products slow down while another kernel (a stand-in for an RCCL
 all-reduce overlapped with the backward) holds some compute units.
-Usage (on the GPU box): python tools/cu_occupancy_bench.py"""
+Usage (on an MI355X): python tools/cu_occupancy_bench.py"""
 import ctypes
 import os
 import sys

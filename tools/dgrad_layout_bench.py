@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Data-gradient products dX = dY W with W [out, in] as stored (reduction-major second operand, read back through the
 transposing LDS read) against the same product on a transposed copy W^T [in, out] (row-major second operand).
-Usage (GPU box): python tools/dgrad_layout_bench.py"""
+Usage (on an MI355X): python tools/dgrad_layout_bench.py"""
 import os
 import sys
 

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Throughput of the training loop fed from a device-resident processed dataset (strided batch
 views, decoder.py:157-166) next to the same steps on a fixed joined batch.
-Usage (GPU box): python tools/epoch_bench.py [samples] [batch]"""
+Usage (on an MI355X): python tools/epoch_bench.py [samples] [batch]"""
 import os
 import sys
 import time

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """What k-panel images of the operands would give the large row-major forward products of the blocks (the persistent
 kernel's standard epilogue): the images are handed in through the diagnostic override of head_fwd.hip, results compared
-bit for bit.  Usage (on the GPU box): python tools/fwd_gemm_panels_probe.py"""
+bit for bit.  Usage (on an MI355X): python tools/fwd_gemm_panels_probe.py"""
 import sys, os, ctypes, torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from image_caption_amd import _lib, ops

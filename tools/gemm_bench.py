@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Micro-benchmark of the GEMM shapes one training step at batch 256 launches.
-Usage (on the GPU box): python tools/gemm_bench.py [reps]"""
+Usage (on an MI355X): python tools/gemm_bench.py [reps]"""
 import os
 import sys
 

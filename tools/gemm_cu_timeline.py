@@ -2,7 +2,7 @@
 """Per-CU phase overlap of the vocabulary-stage forward kernel, from the in-kernel clock stamps:
 how much of a compute unit's time has its two resident workgroups both in the main loop, one in the main
 loop and one in the epilogue, both in the epilogue, or fewer than two workgroups resident.
-Usage (on the GPU box): python tools/gemm_cu_timeline.py"""
+Usage (on an MI355X): python tools/gemm_cu_timeline.py"""
 import ctypes
 import os
 import sys

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Greedy decoding time per token at serving batch sizes: one composed capdec_decode_step call per token
 against the same kernels launched one by one from Python.
-Usage (on the GPU box): python tools/greedy_latency.py"""
+Usage (on an MI355X): python tools/greedy_latency.py"""
 import os
 import sys
 import time

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Timing of the vocabulary stage's two backward products at batch 256 under forced kernel choices
 (capdecdbg_gemm_mode): data gradient 8192 x 768 over 50304 (split-K through a workspace) and weight gradient
-50260 x 768 over 8192.  Usage (on the GPU box): python tools/head_gemm_modes.py [modes...]"""
+50260 x 768 over 8192.  Usage (on an MI355X): python tools/head_gemm_modes.py [modes...]"""
 import ctypes
 import os
 import sys

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Timing of the vocabulary stage's two backward products at batch 256 with d(logits) read as a row-major matrix
 against the same launches reading it as a column-panel image [V/32][M][32] (the values are not rearranged here: timing
-only).  Usage (on the GPU box): python tools/head_gemm_panel_ab.py"""
+only).  Usage (on an MI355X): python tools/head_gemm_panel_ab.py"""
 import ctypes
 import os
 import sys

@@ -3,7 +3,7 @@
 the fused logits + cross-entropy forward (8192 x 50260 x 768, numerators kept) and the vendor library's bare product of
 the same shape (torch.matmul -> hipBLASLt, bf16 output, no loss), each on training-like random operands and on all-zero
 operands (same instruction stream, almost no switching activity in the multipliers), plus the library's 8192^3.
-Diagnostic only: nothing in the package calls torch.matmul.   Usage (on the GPU box): python tools/head_power_probe.py"""
+Diagnostic only: nothing in the package calls torch.matmul.   Usage (on an MI355X): python tools/head_power_probe.py"""
 import os
 import sys
 

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """The backward products of the block on the 8192 scored rows (batch 256), each alone, under forced kernel choices
 (capdecdbg_gemm_mode: 0 default, 1 register-staged, 2 ring 128x128, 4 ring 256x128, 5 ring 256x256, 6 pipelined 256x256,
-7 pipelined 256x128).  Usage (on the GPU box): python tools/mlp_bwd_gemm_bench.py"""
+7 pipelined 256x128).  Usage (on an MI355X): python tools/mlp_bwd_gemm_bench.py"""
 import ctypes
 import os
 import sys

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """The block products of the one-block step that run on the 8192 scored rows (batch 256), each alone, under the default
 kernel choice and with the persistent kernel forced (capdecdbg_gemm_mode 10 / 11: 256x256 / 256x128 tiles).
-Usage (on the GPU box): python tools/mlp_gemm_bench.py"""
+Usage (on an MI355X): python tools/mlp_gemm_bench.py"""
 import ctypes
 import os
 import sys

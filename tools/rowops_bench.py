@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Micro-benchmark of the HBM-bound row kernels of one training step at batch 256, each with
-the bytes it must move and the bandwidth that implies.  Usage (GPU box): python tools/rowops_bench.py"""
+the bytes it must move and the bandwidth that implies.  Usage (on an MI355X): python tools/rowops_bench.py"""
 import os
 import sys
 

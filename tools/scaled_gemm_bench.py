@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Micro-benchmark of the GEMM shapes of one block of the 12-block / 257-patch configuration at batch 256
 (74240 rows): forward, data-gradient and weight-gradient products, each as the engine launches it.
-Usage (on the GPU box): python tools/scaled_gemm_bench.py [reps] [gemm mode] [0: without the persistent pipelined kernel]"""
+Usage (on an MI355X): python tools/scaled_gemm_bench.py [reps] [gemm mode] [0: without the persistent pipelined kernel]"""
 import ctypes
 import os
 import sys

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Soak test: many training steps at the benchmark configuration, looking for a non-finite loss (a rare race
-would show as one).  Usage (on the GPU box): python tools/soak_train.py [steps] [gemm mode]"""
+would show as one).  Usage (on an MI355X): python tools/soak_train.py [steps] [gemm mode]"""
 import ctypes
 import os
 import sys

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """How long a fresh process takes to reach its steady step time: the step time of consecutive groups of 5 training
-steps at the bench configuration, from the first step on.  Usage (on the GPU box): python tools/warmup_probe.py"""
+steps at the bench configuration, from the first step on.  Usage (on an MI355X): python tools/warmup_probe.py"""
 import os
 import sys
 import time
