@@ -401,9 +401,15 @@ template <int HD> __device__ __forceinline__ void store_rows(const f32x16 (&acc)
 //   forward, f32, 2048 heads, 1 / 32 / 64 rows:        104 | 63      106 | 70      157 | 123
 //   backward, bf16, 2048 heads, 1 / 32 / 64 rows:      75.6 | 70.9   81.6 | 79.0   96.2 | 108.6                  (hd 128, where dQ spills: 179 | 196 at 32)
 //   backward, f32, 2048 heads, 1 / 32 / 64 rows:       410 | 371     421 | 398     570 | 593                     (hd 96: 640 | 467 at 32, 773 | 735 at 64)
+//   64 rows in bf16, hd 64 (causal), 256 / 320 / 512 / 768 / 2048 heads: 229 keys  8.5 | 8.2  10.2 | 9.8  11.2 | 13.9  14.3 | 17.8  31.7 | 38.1
+//     1024 keys  43 | 17  52 | 21  26 | 30  36 | 38  111 | 126;  4096 keys  74 | 49  98 | 76  105 | 134  151 | 170  407 | 433
+//     (backward, 1024 keys: 58 | 52  71 | 63  90 | 89  130 | 143  371 | 380)
 //   tiles of 128 rows on 16 CUs (2 x 8 heads of 229 rows, hd 96): 9.0 | 7.9, on 64 (1 head, 8192 rows, hd 128): 48.6 | 30.1,
 //   on 128: 9.3 | 10.2 and 19.8 | 16.4, on 256: 9.9 | 17.9 and 19.5 | 19.8
-inline bool win_few_rows(bool f32, long bh, long rows) { return rows <= (f32 ? 64 : 32) || bh * ((rows + 127) / 128) < 256; }
+// So: up to 32 rows (f32: 64) always; up to 64 while their tiles do not give every CU two workgroups; more while they do not give it one.
+inline bool win_few_rows(bool f32, long bh, long rows) {
+    return rows <= (f32 ? 64 : 32) || bh * ((rows + 127) / 128) < (rows <= 64 ? 512 : 256);
+}
 int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what);
 struct WinFwdPlan { int kw; int tiles; int nsplit; long part_floats; };   // kw: four waves share the keys of 32 rows (else 4 x 32 rows)
 WinFwdPlan win_fwd_plan(bool f32, int B, int H, int Hkv, int S, int nq, int hd, int window, int prefix);

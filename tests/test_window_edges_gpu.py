@@ -283,3 +283,21 @@ def test_a_query_that_sees_one_key_has_no_gradient_for_its_score(case, dtype):
     assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
     for got, (want, bound), what in zip((dq, dk, dv), wo.backward(q, k, v, o, lse, dout, see, 1.0), ("dq", "dk", "dv")):
         wo.assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("B,H,Hkv,S,nq,hd", [(64, 8, 8, 300, 40, 64), (65, 16, 8, 200, 20, 32), (63, 8, 8, 700, 64, 128), (32, 16, 8, 1500, 30, 96)])
+def test_rows_between_the_shapes_with_two_workgroups_for_a_cu(B, H, Hkv, S, nq, hd):
+    """33..64 rows in bf16 on either side of 512 K/V heads."""
+    print(B, H, Hkv, S, nq, hd, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(31)
+    q, dout = ((torch.randn(B, H, nq, hd, generator=g, device=DEV) * x).bfloat16() for x in (hd ** -0.5, 1.0))
+    k, v = (torch.randn(B, Hkv, S, hd, generator=g, device=DEV).bfloat16() for _ in range(2))
+    kw = dict(window=0, prefix_len=0, q_start=S - nq)
+    o, lse, *grads = run(q, k, v, dout, **kw)
+    for b in range(0, B, 16):
+        part = slice(b, min(B, b + 16))
+        see = wo.masks(part.stop - part.start, S, nq, S - nq, [S] * (part.stop - part.start), 0, 0, False, DEV)
+        want, _, bound, _ = wo.forward(q[part], k[part], v[part], see)
+        wo.assert_within(o[part], want, bound, "o")
+        for got, (w, bd), what in zip(grads, wo.backward(q[part], k[part], v[part], o[part], lse[part], dout[part], see, 1.0), ("dq", "dk", "dv")):
+            wo.assert_within(got[part], w, bd, what)
