@@ -36,7 +36,8 @@ constexpr int KT = 128;              // keys of a dK / dV workgroup: four waves 
 constexpr int RB = 32;               // rows per step
 
 // The common part c of the keys, for dQ: the mean of m keys spread over the longer run of visible ones, in the channels where it stands out
-// of the keys' own spread (five standard errors of that mean: what is below would only be the sample's noise).  One key in sixteen,
+// of the keys' own spread (six standard errors of that mean: what is below would only be the sample's
+// noise, and of keys without a common part one channel in 10^6 or 10^7 passes by chance).  One key in sixteen,
 // 64 at least and 1024 at most: what is left of c costs dQ less than its roundings do with 64 keys up to about a thousand,
 // and dQ, a mean over n keys, shrinks like 1 / sqrt(n) against it (100 rows over 10000 keys, 0.0074 of dQ with 64).  Fewer than 32
 // keys say nothing: c = 0.  Formed at the start of a workgroup; partial sums and squares meet in LDS.
@@ -95,7 +96,7 @@ template <int HD, int NT> struct KeyMean {
             s2 += y[1];
         }
         const float inv = 1.f / (float)max(m, 1), mean = s * inv, var = fmaxf(fmaf(-mean, mean, s2 * inv), 0.f);
-        *reinterpret_cast<float*>(lds + PART + 4 * tid) = m >= 32 && (float)m * mean * mean > 25.f * var ? mean : 0.f;
+        *reinterpret_cast<float*>(lds + PART + 4 * tid) = m >= 32 && (float)m * mean * mean > 36.f * var ? mean : 0.f;
     }
     static __device__ __forceinline__ f32x4 at(const char* lds, int channel) { return *reinterpret_cast<const f32x4*>(lds + PART + 4 * channel); }
 };
