@@ -269,8 +269,8 @@ int capdec_attn_window_fwd(const capdec_attn_window_desc* desc, void* stream);
  * delta [B*H*nq] f32 scratch.  fwd.workspace: capdec_attn_window_bwd_workspace(...) bytes, required unless that is 0 (it
  * covers either dtype; bf16 calls over at most 256 keys that one kernel runs take none).
  * No atomics: the same call gives the same bits.  bf16: P and dS are rounded once to be operands and delta = sum dO o carries
- * o's rounding; dQ is freed of what that and a common part of the keys would make together (0.0024-0.0038 of its size
- * at any offset; a common part of V is left in delta, 0.005 at twice V's spread). */
+ * o's rounding; dQ is freed of what that and a common part of the keys would make together (0.0024-0.0033 of its size
+ * at any offset up to about a thousand keys; a common part of V is left in delta, 0.005 at twice V's spread). */
 typedef struct {
     capdec_attn_window_desc fwd;
     const void* dout; long do_bs, do_hs, do_ss;
