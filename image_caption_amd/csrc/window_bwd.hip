@@ -17,7 +17,7 @@
 // 0.009 and 0.035 of its size off.  In exact numbers the sum is 0 and any c may be taken out of the keys, so
 //     dQ = sum_j dS_j K_j - (sum_j dS_j) c,     the sum over the rounded dS, c the common part of some of the visible keys
 // (KeyMean below): one number a row, a 2-term dot product per two elements of dS.  dQ then lies 0.0024-0.0033 of its size from the exact one
-// whatever the offset (0.004-0.005 as a mean over 5000-10000 keys), dK 0.0024-0.0025, dV 0.0023, against 0.0017 for their own rounding alone.  Cost: captioning stack 123.0 -> 127.6 us, 3 of
+// whatever the offset (0.004-0.005 as a mean over 5000-10000 keys), dK 0.0024-0.0029, dV 0.0023, against 0.0017 for their own rounding alone.  Cost: captioning stack 123.0 -> 127.6 us, 3 of
 // them the dot products (sums by matrix instructions against ones: 128.3), 8192 positions 318 -> 321, 100 rows over 10000 keys 98 -> 109.
 // What V's rows have in common reaches delta through o's rounding, stays in the formula and is left: 0.005 of dQ and dK for an offset of
 // twice V's spread, 0.02 for eight times, and 0.005 of dQ where 9000 keys are averaged over an offset of a quarter.  An exact delta, 0.0023-0.0026,
