@@ -286,14 +286,13 @@ int win_fill(const capdec_attn_window_desc* d, WinArgs& a, const char* what) {
                  (long)d->q_start + d->nq, d->S);
     CAPDEC_CHECK(d->window >= 0 && d->prefix_len >= 0, "%s: window %d, prefix %d", what, d->window, d->prefix_len);
     const int G = d->H / d->Hkv;
-    CAPDEC_CHECK((long)d->nq * G * G < (1L << 31) && (long)d->B * d->Hkv < (1L << 31), "%s: %d queries of %d heads to a K/V head", what, d->nq, G);
+    CAPDEC_CHECK((double)d->nq * G * G < 2147483648.0 && (long)d->B * d->Hkv < (1L << 31), "%s: %d queries of %d heads to a K/V head", what, d->nq, G);
     const int e = d->dtype == CAPDEC_BF16 ? 2 : 4, per16 = 16 / e;
     CAPDEC_CHECK(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && aligned16(d->o), "%s: operands must be 16-byte aligned", what);
     const long st[] = {d->q_bs, d->q_hs, d->q_ss, d->k_bs, d->k_hs, d->k_ss, d->v_bs, d->v_hs, d->v_ss, d->o_bs, d->o_hs, d->o_ss};
     for (long s : st) CAPDEC_CHECK(s >= 0 && s % per16 == 0, "%s: stride %ld (must be a non-negative multiple of %d elements)", what, s, per16);
-    // (a buffer's 64 rows are addressed by 31 bits)
-    CAPDEC_CHECK(64L * d->k_ss * e < (1L << 31) && 64L * d->v_ss * e < (1L << 31), "%s: key rows lie too far apart (%ld and %ld bytes, 32 MiB or more)", what,
-                 d->k_ss * e, d->v_ss * e);
+    // (a buffer's 64 rows are addressed by 31 bits; compared by division: a product with a stride of 2^58 wraps)
+    CAPDEC_CHECK(d->k_ss < (1L << 25) / e && d->v_ss < (1L << 25) / e, "%s: key rows lie too far apart (%ld and %ld elements, 32 MiB or more)", what, d->k_ss, d->v_ss);
     memset(&a, 0, sizeof(a));
     a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o;
     a.q_bs = d->q_bs; a.q_hs = d->q_hs; a.q_ss = d->q_ss;

@@ -93,3 +93,29 @@ def test_decode_step_refuses_before_it_advances_the_tokens(four, window):
         assert rc == -1 and text in why, (bad, rc, why)
     rc, why = decode_step(None, last=dict(norm2_b=None))
     assert rc == -1 and "null" in why
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("name", ["k_ss", "v_ss"])
+def test_key_strides_whose_products_wrap_are_refused(name, dtype):
+    """64 or 128 rows of 2^58 elements and more are 0 in 64 bits; nothing of the addresses may reach a launch (-2 here)."""
+    import ctypes
+    from image_caption_amd import _lib
+    from test_window_attention_cpu import bwd_desc, desc
+    lib = _lib.load()
+    code = (_lib.BF16, _lib.F32)[dtype]
+    for stride in (1 << 25, 1 << 56, 1 << 57, 1 << 58, 1 << 60, (1 << 62) + 64):
+        d = desc(dtype=code, **{name: stride})
+        assert lib.capdec_attn_window_fwd(ctypes.byref(d), None) == -1 and b"too far apart" in lib.capdec_last_error(), stride
+        assert lib.capdec_attn_window_bwd(ctypes.byref(bwd_desc(d)), None) == -1 and b"too far apart" in lib.capdec_last_error(), stride
+
+
+def test_more_rows_than_32_bits_are_refused():
+    """16 queries of 2^30 heads on one K/V head: queries * heads * heads is 2^64, which 64 bits hold as 0."""
+    import ctypes
+    from image_caption_amd import _lib
+    from test_window_attention_cpu import bwd_desc, desc
+    lib = _lib.load()
+    d = desc(B=1, H=1 << 30, Hkv=1, nq=16, q_start=48)
+    assert lib.capdec_attn_window_fwd(ctypes.byref(d), None) == -1 and b"queries of" in lib.capdec_last_error()
+    assert lib.capdec_attn_window_bwd(ctypes.byref(bwd_desc(d)), None) == -1 and b"queries of" in lib.capdec_last_error()
